@@ -457,6 +457,60 @@ int skv_attention_ex_noalloc(const skv_attention_desc* desc, skv_stream_t stream
  */
 int skv_noalloc_init(void);
 
+/*
+ * skv_qk_norm_rope — RMS norm of every query and key head with the position rotation in the same
+ * pass (the "qk-norm + RoPE" step of minimax_h3/fused_ops.py:1-16, forward and backward).  Per
+ * token and head, in fp32 with one rounding at the end:
+ *   y = weight . x / sqrt(mean(x^2) + eps)          (norm != 0; weight NULL: ones)
+ *   out = y with its first 2 * half channels turned in pairs by the token's angle: channels
+ *         (2i, 2i + 1) when `interleaved`, (i, i + half) otherwise, by cos / sin column i.
+ * q and k are [batch][rows][heads][128] views of one dtype (F32, BF16, F16) with element strides,
+ * 16-byte aligned, strides non-negative multiples of 8; k.heads = 0 leaves k out.  A weight is
+ * [128] of any of the three types.  cos / sin: f32 [table_rows][half], row stride table_stride (a
+ * multiple of 4), half = 8, 16 .. 64, or NULL and half = 0 for the norm alone.  The table row of a
+ * token is position0 + positions[b * pos_sb + t * pos_st] (int32, or int64 when pos_is_int64), or
+ * position0 + t without `positions`; channels turned by a row outside the table become NaN.
+ * out may be x itself, and must not otherwise overlap any input or output.
+ *
+ * skv_qk_norm_rope_grad — its gradient: `grad` holds dL/d(out), `out` takes dL/dx, and
+ * grad_weight (NULL: not wanted) the weight's gradient, summed over all rows in a fixed order.
+ * It needs the workspace that skv_qk_norm_rope_grad_workspace reports for the same descriptor
+ * (16-byte aligned, used by the launch only).
+ */
+typedef struct skv_norm_side {
+  const void* x;
+  int64_t x_sb, x_st, x_sh;
+  const void* grad;
+  int64_t grad_sb, grad_st, grad_sh;
+  void* out;
+  int64_t out_sb, out_st, out_sh;
+  const void* weight;
+  int weight_dtype;
+  int norm;
+  float eps;
+  int heads;
+  void* grad_weight;
+  int grad_weight_dtype;
+} skv_norm_side;
+
+typedef struct skv_qk_norm_rope_desc {
+  skv_norm_side q, k;
+  int dtype, batch, rows, head_dim;
+  const float* cos;
+  const float* sin;
+  int64_t table_stride, table_rows;
+  int half, interleaved;
+  const void* positions;
+  int pos_is_int64;
+  int64_t pos_sb, pos_st, position0;
+  void* workspace;
+  int64_t workspace_bytes;
+} skv_qk_norm_rope_desc;
+
+int skv_qk_norm_rope(const skv_qk_norm_rope_desc* desc, skv_stream_t stream);
+int skv_qk_norm_rope_grad(const skv_qk_norm_rope_desc* desc, skv_stream_t stream);
+int skv_qk_norm_rope_grad_workspace(const skv_qk_norm_rope_desc* desc, int64_t* bytes /* host */);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,8 @@ Public surface (the reference's call signatures, solar/backends/wan22/runtime):
 * :func:`make_crossattn_cache_allocator`, :func:`cross_attend` — the cross-attention K/V cache
 * ``prope_branch=`` of the allocator, :func:`prope_branch_attention` — the cache of the PRoPE
   self-attention branch (camera_attention_mode "parallel")
+* :func:`qk_norm_rope` — per-head q/k RMS norm with the position rotation in the same pass, and
+  its gradient
 * :mod:`solarwm_amd.driver` — the sampler's pass/commit driver and the block loop
 """
 
@@ -24,6 +26,7 @@ from .attention import (apply_cache_updates, attend_cached, attention, chunk_cau
 from .crossattn import CrossAttnCache, cross_attend, make_crossattn_cache_allocator
 from .cache import CacheGeometry, CachePlan, SlotKVCache, make_kv_cache_allocator, plan_cached_forward
 from .prope import PropeConfig, commit_camera_cache, drop_camera_cache, stage_camera_cache
+from .qknorm import qk_norm_rope
 from .rope import RopeConfig
 
 __all__ = [
@@ -44,5 +47,6 @@ __all__ = [
     "make_kv_cache_allocator",
     "plan_cached_forward",
     "prope_branch_attention",
+    "qk_norm_rope",
     "stage_camera_cache",
 ]

@@ -100,6 +100,31 @@ class PropeStageDesc(ctypes.Structure):
     ]
 
 
+class NormSide(ctypes.Structure):
+    """``skv_norm_side`` (include/solarkv.h), field for field."""
+
+    _fields_ = [
+        ("x", _vp), ("x_sb", _i64), ("x_st", _i64), ("x_sh", _i64),
+        ("grad", _vp), ("grad_sb", _i64), ("grad_st", _i64), ("grad_sh", _i64),
+        ("out", _vp), ("out_sb", _i64), ("out_st", _i64), ("out_sh", _i64),
+        ("weight", _vp), ("weight_dtype", _i32), ("norm", _i32), ("eps", _f32), ("heads", _i32),
+        ("grad_weight", _vp), ("grad_weight_dtype", _i32),
+    ]
+
+
+class QkNormRopeDesc(ctypes.Structure):
+    """``skv_qk_norm_rope_desc`` (include/solarkv.h), field for field."""
+
+    _fields_ = [
+        ("q", NormSide), ("k", NormSide),
+        ("dtype", _i32), ("batch", _i32), ("rows", _i32), ("head_dim", _i32),
+        ("cos", _vp), ("sin", _vp), ("table_stride", _i64), ("table_rows", _i64),
+        ("half", _i32), ("interleaved", _i32),
+        ("positions", _vp), ("pos_is_int64", _i32), ("pos_sb", _i64), ("pos_st", _i64),
+        ("position0", _i64), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 class LaunchPlan(ctypes.Structure):
     """``skv_launch_plan`` (include/solarkv.h): the launch skv_attention_ex would make."""
 
@@ -160,6 +185,10 @@ SIGNATURES: dict[str, tuple] = {
     "skv_noalloc_init": (_i32, []),
     "skv_append_workspace_size": (_i32, [ctypes.POINTER(AppendDesc), ctypes.POINTER(_i64)]),
     "skv_prope_stage": (_i32, [ctypes.POINTER(PropeStageDesc), _vp]),
+    "skv_qk_norm_rope": (_i32, [ctypes.POINTER(QkNormRopeDesc), _vp]),
+    "skv_qk_norm_rope_grad": (_i32, [ctypes.POINTER(QkNormRopeDesc), _vp]),
+    "skv_qk_norm_rope_grad_workspace": (_i32, [ctypes.POINTER(QkNormRopeDesc),
+                                               ctypes.POINTER(_i64)]),
     "skv_h3_rope_prope": (_i32, [ctypes.POINTER(H3XformDesc), _vp]),
 }
 
