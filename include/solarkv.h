@@ -511,6 +511,100 @@ int skv_qk_norm_rope(const skv_qk_norm_rope_desc* desc, skv_stream_t stream);
 int skv_qk_norm_rope_grad(const skv_qk_norm_rope_desc* desc, skv_stream_t stream);
 int skv_qk_norm_rope_grad_workspace(const skv_qk_norm_rope_desc* desc, int64_t* bytes /* host */);
 
+/*
+ * Sequences that share a history.  A page is a frame slot with a batch of one: K pool
+ * [n_pages][H][Tp][128], V pool [n_pages][H][128][Tp] (bf16 or f16), page_tokens = T tokens of it in
+ * use, Tp = T rounded up to 64.  A sequence's token i lies at offset i % T of page
+ * tables[b * table_stride + i / T] (device int32, table_width entries a sequence); an entry outside
+ * [0, n_pages) is a page that is not there.  lengths[b] (device int32) counts a sequence's own tokens
+ * with this call's new ones; new_lens[b] (device int32, NULL: every row) says how many of the call's
+ * `rows` rows are new tokens of it, row t being token lengths[b] - new_lens[b] + t.
+ *
+ * skv_append_pages — new K and V into their pages, K normalised per head and rotated on the way
+ * (as skv_qk_norm_rope), and the queries with them into q_out (q_heads = 0 leaves them out).  The
+ * table row of a token's rotation is position0 + positions[b][t], or without `positions`
+ * position0 + its own index (position0 = tokens of the shared prefix).  Rows that are no new tokens
+ * and tokens without a page write no K and V; q_out rows that are no new tokens are zero.  A page is
+ * written by one sequence of a call (two tokens of one place leave either's values).
+ * (Replaces the scatter of normalised, rotated K and of V into a pooled cache,
+ * deploy/solar_wm/shared/vae/streamrender_tp.py:21-60.)
+ */
+typedef struct skv_head_norm {
+  const void* weight; /* [128] f32, bf16 or f16; NULL: ones */
+  int weight_dtype;
+  int norm; /* 0: no norm */
+  float eps;
+} skv_head_norm;
+
+typedef struct skv_append_pages_desc {
+  const void* k;
+  int64_t k_sb, k_st, k_sh;
+  const void* v;
+  int64_t v_sb, v_st, v_sh;
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  void* q_out;
+  int64_t out_sb, out_st, out_sh;
+  void* k_pool;
+  void* v_pool;
+  int dtype, n_pages, page_tokens, batch, rows, q_heads, kv_heads, head_dim;
+  const int32_t* tables;
+  int64_t table_stride;
+  int table_width;
+  const int32_t* lengths;
+  const int32_t* new_lens;
+  skv_head_norm norm_q, norm_k;
+  const float* cos;
+  const float* sin;
+  int64_t cos_stride, table_rows;
+  int half, interleaved;
+  const void* positions;
+  int pos_is_int64;
+  int64_t pos_sb, pos_st, position0;
+} skv_append_pages_desc;
+
+int skv_append_pages(const skv_append_pages_desc* desc, skv_stream_t stream);
+
+/*
+ * skv_attend_shared — attention of a batch whose sequences all see one prefix (prefix_tokens tokens
+ * in prefix_pages, of these pools or of others) and then their own pages:
+ *   out = softmax(q [k_prefix, k_own]^T * softmax_scale) [v_prefix, v_own]
+ * with q and out [batch][rows][q_heads][128] views (16-byte aligned, strides non-negative multiples
+ * of 8) and q_heads a multiple of kv_heads.  `causal`: row t of a sequence sees its first
+ * lengths[b] - new_lens[b] + t + 1 own tokens; otherwise all lengths[b].  Keys of pages that are not
+ * there are not seen; a row that sees no key, and rows that are no new tokens, are zero.  What pages
+ * hold behind their tokens does not matter, infinities and NaN included.  bf16 / f16 matrix-core
+ * products with fp32 accumulation and an fp32 online softmax; every part of the keys leaves fp32
+ * partial results in the workspace that skv_attend_shared_workspace reports for the same descriptor
+ * (16-byte aligned, used by the call only), joined in a fixed order.
+ */
+typedef struct skv_attend_shared_desc {
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  void* out;
+  int64_t out_sb, out_st, out_sh;
+  const void* k_pool;
+  const void* v_pool;
+  int dtype, n_pages, page_tokens, batch, rows, q_heads, kv_heads, head_dim;
+  const int32_t* tables;
+  int64_t table_stride;
+  int table_width;
+  const int32_t* lengths;
+  const int32_t* new_lens;
+  const void* prefix_k_pool;
+  const void* prefix_v_pool;
+  int prefix_n_pages, prefix_page_tokens;
+  const int32_t* prefix_pages; /* device, ceil(prefix_tokens / prefix_page_tokens) entries */
+  int64_t prefix_tokens;
+  int causal;
+  float softmax_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} skv_attend_shared_desc;
+
+int skv_attend_shared(const skv_attend_shared_desc* desc, skv_stream_t stream);
+int skv_attend_shared_workspace(const skv_attend_shared_desc* desc, int64_t* bytes /* host */);
+
 #ifdef __cplusplus
 }
 #endif

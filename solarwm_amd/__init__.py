@@ -18,6 +18,9 @@ Public surface (the reference's call signatures, solar/backends/wan22/runtime):
   self-attention branch (camera_attention_mode "parallel")
 * :func:`qk_norm_rope` — per-head q/k RMS norm with the position rotation in the same pass, and
   its gradient
+* :func:`append_pages`, :func:`attend_shared`, :func:`history_pages` — sequences that share a
+  history: new tokens into paged caches (norm and rotation on the way), and attention over one
+  prefix for the whole batch and each sequence's own pages
 * :mod:`solarwm_amd.driver` — the sampler's pass/commit driver and the block loop
 """
 
@@ -25,6 +28,7 @@ from .attention import (apply_cache_updates, attend_cached, attention, chunk_cau
                         prope_branch_attention)
 from .crossattn import CrossAttnCache, cross_attend, make_crossattn_cache_allocator
 from .cache import CacheGeometry, CachePlan, SlotKVCache, make_kv_cache_allocator, plan_cached_forward
+from .paged import append_pages, attend_shared, history_pages
 from .prope import PropeConfig, commit_camera_cache, drop_camera_cache, stage_camera_cache
 from .qknorm import qk_norm_rope
 from .rope import RopeConfig
@@ -36,13 +40,16 @@ __all__ = [
     "PropeConfig",
     "RopeConfig",
     "SlotKVCache",
+    "append_pages",
     "apply_cache_updates",
     "attend_cached",
+    "attend_shared",
     "attention",
     "chunk_causal_attention",
     "commit_camera_cache",
     "cross_attend",
     "drop_camera_cache",
+    "history_pages",
     "make_crossattn_cache_allocator",
     "make_kv_cache_allocator",
     "plan_cached_forward",

@@ -125,6 +125,50 @@ class QkNormRopeDesc(ctypes.Structure):
     ]
 
 
+class HeadNorm(ctypes.Structure):
+    """``skv_head_norm`` (include/solarkv.h), field for field."""
+
+    _fields_ = [("weight", _vp), ("weight_dtype", _i32), ("norm", _i32), ("eps", _f32)]
+
+
+class AppendPagesDesc(ctypes.Structure):
+    """``skv_append_pages_desc`` (include/solarkv.h), field for field."""
+
+    _fields_ = [
+        ("k", _vp), ("k_sb", _i64), ("k_st", _i64), ("k_sh", _i64),
+        ("v", _vp), ("v_sb", _i64), ("v_st", _i64), ("v_sh", _i64),
+        ("q", _vp), ("q_sb", _i64), ("q_st", _i64), ("q_sh", _i64),
+        ("q_out", _vp), ("out_sb", _i64), ("out_st", _i64), ("out_sh", _i64),
+        ("k_pool", _vp), ("v_pool", _vp),
+        ("dtype", _i32), ("n_pages", _i32), ("page_tokens", _i32), ("batch", _i32), ("rows", _i32),
+        ("q_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+        ("tables", _vp), ("table_stride", _i64), ("table_width", _i32),
+        ("lengths", _vp), ("new_lens", _vp), ("norm_q", HeadNorm), ("norm_k", HeadNorm),
+        ("cos", _vp), ("sin", _vp), ("cos_stride", _i64), ("table_rows", _i64),
+        ("half", _i32), ("interleaved", _i32),
+        ("positions", _vp), ("pos_is_int64", _i32), ("pos_sb", _i64), ("pos_st", _i64),
+        ("position0", _i64),
+    ]
+
+
+class AttendSharedDesc(ctypes.Structure):
+    """``skv_attend_shared_desc`` (include/solarkv.h), field for field."""
+
+    _fields_ = [
+        ("q", _vp), ("q_sb", _i64), ("q_st", _i64), ("q_sh", _i64),
+        ("out", _vp), ("out_sb", _i64), ("out_st", _i64), ("out_sh", _i64),
+        ("k_pool", _vp), ("v_pool", _vp),
+        ("dtype", _i32), ("n_pages", _i32), ("page_tokens", _i32), ("batch", _i32), ("rows", _i32),
+        ("q_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+        ("tables", _vp), ("table_stride", _i64), ("table_width", _i32),
+        ("lengths", _vp), ("new_lens", _vp),
+        ("prefix_k_pool", _vp), ("prefix_v_pool", _vp),
+        ("prefix_n_pages", _i32), ("prefix_page_tokens", _i32),
+        ("prefix_pages", _vp), ("prefix_tokens", _i64), ("causal", _i32), ("softmax_scale", _f32),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 class LaunchPlan(ctypes.Structure):
     """``skv_launch_plan`` (include/solarkv.h): the launch skv_attention_ex would make."""
 
@@ -189,6 +233,9 @@ SIGNATURES: dict[str, tuple] = {
     "skv_qk_norm_rope_grad": (_i32, [ctypes.POINTER(QkNormRopeDesc), _vp]),
     "skv_qk_norm_rope_grad_workspace": (_i32, [ctypes.POINTER(QkNormRopeDesc),
                                                ctypes.POINTER(_i64)]),
+    "skv_append_pages": (_i32, [ctypes.POINTER(AppendPagesDesc), _vp]),
+    "skv_attend_shared": (_i32, [ctypes.POINTER(AttendSharedDesc), _vp]),
+    "skv_attend_shared_workspace": (_i32, [ctypes.POINTER(AttendSharedDesc), ctypes.POINTER(_i64)]),
     "skv_h3_rope_prope": (_i32, [ctypes.POINTER(H3XformDesc), _vp]),
 }
 

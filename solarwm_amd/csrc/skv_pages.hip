@@ -1,0 +1,973 @@
+// Sequences that share a history: new tokens into a paged cache (skv_append_pages) and attention of
+// a batch whose sequences all see one prefix and then pages of their own (skv_attend_shared).
+//
+// A page is a frame slot with a batch of one: K [pages][H][Tp][128], V [pages][H][128][Tp], T
+// tokens of a page in use (Tp = T rounded up to 64).  A sequence's token i lies at offset i % T of
+// page tables[b][i / T]; page numbers outside the pool are pages that are not there: nothing is
+// written to them and their keys are not seen.
+#include "skv_rowops.h"
+
+namespace skv {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------------------------
+struct Pages {
+  const int32_t* tables;
+  int64_t table_st;
+  int width, n_pages, T, Tp, heads;
+  const int32_t* lengths;
+  const int32_t* new_lens;
+
+  // tokens of sequence b with the new ones, and the new ones among its `rows` rows
+  __device__ int fresh(int b, int rows) const {
+    if (new_lens == nullptr) return rows;
+    const int n = new_lens[b];
+    return n < 0 ? 0 : n > rows ? rows : n;
+  }
+  __device__ int64_t first(int b, int n) const { return (int64_t)lengths[b] - n; }
+};
+
+struct AppendPagesArgs {
+  Pages pg;
+  const void *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  void* q_out;
+  int64_t o_sb, o_st, o_sh;
+  void *k_pool, *v_pool;
+  const void *wq, *wk;
+  int wq_dtype, wk_dtype, norm_q, norm_k, q_heads, q_blocks, k_blocks;
+  float eps_q, eps_k;
+  const float *cos, *sin;
+  int64_t tab_st, tab_rows;
+  const void* pos;
+  int64_t pos_sb, pos_st, pos0;
+  int pos64, half, batch, rows;
+  int n_units_q, n_units, n_unit_groups;  // (token, head block) units of q and of q and k
+  int v_tiles;                            // per (sequence, head); 0: a wave per token instead
+};
+
+// The page row of a sequence's token `own`: its row in [pages][T], or -1 where there is none.
+__device__ inline int64_t page_of(const Pages& pg, int b, int64_t own, int* off) {
+  if (own < 0) return -1;
+  const int64_t p = own / pg.T;
+  if (p >= pg.width) return -1;
+  *off = (int)(own - p * pg.T);
+  const int id = pg.tables[b * pg.table_st + p];
+  return id < 0 || id >= pg.n_pages ? -1 : id;
+}
+
+// V of one token and head by one wave: a lane's two channels go to two rows of the page.
+template <typename T>
+__device__ inline void v_token(const AppendPagesArgs& a, int unit) {
+  const int lane = threadIdx.x & 63;
+  const int h = unit % a.pg.heads, bl = unit / a.pg.heads;
+  const int row = bl % a.rows, b = bl / a.rows;
+  if (b >= a.batch) return;
+  const int n = a.pg.fresh(b, a.rows);
+  if (row >= n) return;
+  int off = 0;
+  const int64_t page = page_of(a.pg, b, a.pg.first(b, n) + row, &off);
+  if (page < 0) return;
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(
+      static_cast<const T*>(a.v) + b * a.v_sb + row * a.v_st + h * a.v_sh + 2 * lane);
+  uint16_t* o = static_cast<uint16_t*>(a.v_pool) +
+                ((page * a.pg.heads + h) * kHeadDim + 2 * lane) * (int64_t)a.pg.Tp + off;
+  o[0] = (uint16_t)w;
+  o[a.pg.Tp] = (uint16_t)(w >> 16);
+}
+
+// V of the tokens that one 64-token tile of a page takes: rows in through LDS, out as pieces of 8
+// tokens of a channel (16 B) where all 8 are new, token by token at the ends.
+template <typename T>
+__device__ inline void v_tile(const AppendPagesArgs& a, int unit, uint32_t (&buf)[kTile][65]) {
+  const int j = unit % a.v_tiles, bh = unit / a.v_tiles;
+  const int h = bh % a.pg.heads, b = bh / a.pg.heads;
+  const int n = a.pg.fresh(b, a.rows);
+  const int64_t o0 = a.pg.first(b, n), o1 = o0 + n, from = o0 > 0 ? o0 : 0;
+  if (from >= o1) return;
+  const int per_page = (a.pg.T + kTile - 1) / kTile;
+  const int64_t p0 = from / a.pg.T;
+  const int64_t tile = p0 * per_page + (from - p0 * a.pg.T) / kTile + j;
+  const int64_t p = tile / per_page;
+  const int t0 = (int)(tile - p * per_page) * kTile;  // first token of the tile in its page
+  const int64_t base = p * a.pg.T + t0;               // its own index
+  const int cap = a.pg.T - t0 < kTile ? a.pg.T - t0 : kTile;
+  const int lo = from > base ? (int)(from - base) : 0;
+  const int hi = o1 - base < cap ? (int)(o1 - base) : cap;
+  if (lo >= hi || p >= a.pg.width) return;
+  const int id = a.pg.tables[b * a.pg.table_st + p];
+  if (id < 0 || id >= a.pg.n_pages) return;
+  const int tid = threadIdx.x, c = tid & 15;
+  const T* v = static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh + 8 * c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (tid >> 4) + 16 * i;
+    if (r >= lo && r < hi) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(v + (base + r - o0) * a.v_st);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) buf[r][4 * c + e] = w[e];
+    }
+  }
+  __syncthreads();
+  uint16_t* o = static_cast<uint16_t*>(a.v_pool) +
+                ((int64_t)id * a.pg.heads + h) * kHeadDim * (int64_t)a.pg.Tp + t0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int piece = tid & 7, pair = (tid >> 3) + 32 * i;  // 8 tokens of channels 2 pair, 2 pair + 1
+    const int r0 = 8 * piece;
+    if (r0 >= hi || r0 + 8 <= lo) continue;
+    u32x4 even, odd;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = buf[r0 + 2 * e][pair], y = buf[r0 + 2 * e + 1][pair];
+      even[e] = (x & 0xffffu) | (y << 16);
+      odd[e] = (x >> 16) | (y & 0xffff0000u);
+    }
+    uint16_t* p0w = o + (int64_t)(2 * pair) * a.pg.Tp + r0;
+    uint16_t* p1w = p0w + a.pg.Tp;
+    if (r0 >= lo && r0 + 8 <= hi) {
+      *reinterpret_cast<u32x4*>(p0w) = even;
+      *reinterpret_cast<u32x4*>(p1w) = odd;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (r0 + e >= lo && r0 + e < hi) {
+          p0w[e] = (uint16_t)(even[e / 2] >> (16 * (e & 1)));
+          p1w[e] = (uint16_t)(odd[e / 2] >> (16 * (e & 1)));
+        }
+    }
+  }
+}
+
+// Workgroups [0, n_unit_groups): 16 (token, head block) units each of q and then of k; the rest:
+// V, a tile of a page or four tokens each.
+template <typename T, bool INTER>
+__global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
+  __shared__ uint32_t buf[kTile][65];
+  if ((int)blockIdx.x >= a.n_unit_groups) {
+    const int g = (int)blockIdx.x - a.n_unit_groups;
+    if (a.v_tiles) v_tile<T>(a, g, buf);
+    else v_token<T>(a, g * 4 + (threadIdx.x >> 6));
+    return;
+  }
+  const int lane64 = threadIdx.x & 63, c = 8 * (lane64 & 15);
+  int unit = (int)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const TurnLane<INTER> lane(a.half, lane64);
+  const bool live = unit < a.n_units;
+  const bool is_q = live && unit < a.n_units_q;
+  unit = !live ? 0 : is_q ? unit : unit - a.n_units_q;
+  const int blocks = is_q ? a.q_blocks : a.k_blocks, heads = is_q ? a.q_heads : a.pg.heads;
+  const int h0 = unit % blocks * kHeadBlock, bl = unit / blocks;
+  const int row = bl % a.rows, b = bl / a.rows;
+  const int64_t st = is_q ? a.q_sh : a.k_sh;
+  const T* x = is_q ? static_cast<const T*>(a.q) + b * a.q_sb + row * a.q_st
+                    : static_cast<const T*>(a.k) + b * a.k_sb + row * a.k_st;
+  const int n = a.pg.fresh(b, a.rows);
+  const bool token = live && row < n;
+  Raw8<T> raw[kHeadBlock];
+#pragma unroll
+  for (int i = 0; i < kHeadBlock; ++i)
+    raw[i] = token && h0 + i < heads ? Raw8<T>::load(x + (h0 + i) * st + c) : Raw8<T>::zero();
+  const int64_t own = a.pg.first(b, n) + row;
+  int64_t pos = a.pos0 + own;
+  if (a.pos != nullptr) {
+    const int64_t i = b * a.pos_sb + row * a.pos_st;
+    pos = a.pos0 + (a.pos64 ? static_cast<const int64_t*>(a.pos)[i]
+                            : (int64_t)static_cast<const int32_t*>(a.pos)[i]);
+  }
+  Turn<INTER> turn;
+  turn.load(a.cos, a.sin, a.tab_st, a.tab_rows, pos, lane);
+  const void* wt = is_q ? a.wq : a.wk;
+  const int wd = is_q ? a.wq_dtype : a.wk_dtype;
+  float w[8], wp[8];
+  load_weight8(wt, wd, c, w);
+  if constexpr (!INTER) load_weight8(wt, wd, 8 * (lane.partner & 15), wp);
+  T* o = nullptr;
+  int64_t oh = 0;
+  if (is_q) {
+    o = static_cast<T*>(a.q_out) + b * a.o_sb + row * a.o_st;
+    oh = a.o_sh;
+  } else if (token) {
+    int off = 0;
+    const int64_t page = page_of(a.pg, b, own, &off);
+    if (page >= 0) o = static_cast<T*>(a.k_pool) + (page * a.pg.heads * a.pg.Tp + off) * kHeadDim;
+    oh = (int64_t)a.pg.Tp * kHeadDim;
+  }
+  const bool norm = is_q ? a.norm_q : a.norm_k;
+  const float eps = is_q ? a.eps_q : a.eps_k;
+#pragma unroll
+  for (int i = 0; i < kHeadBlock; ++i) {
+    Raw8<T> z = norm_turn<T, INTER>(raw[i], norm, eps, w, wp, turn, lane);
+    if (!token) z = Raw8<T>::zero();  // rows behind a sequence's new tokens
+    if (o != nullptr && live && h0 + i < heads) z.store(o + (h0 + i) * oh + c);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// attention
+//
+// With G = query heads per key head, row m = (b * L + l) * G + g of key head h is query (b, l, h G
+// + g).  The prefix's scores are products of its keys with ALL rows of a key head, so its K and V
+// are read once for the batch (once per row block); a sequence's own pages meet its own L * G rows.
+// Both are split along the keys; every part leaves per row its maximum m, its sum l of exp2(s - m)
+// and its unnormalised fp32 output, which merge_kernel joins:
+//   out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p,  m = max m_p.
+//
+// A wave works on 16 R rows and 32 keys a step: S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs.
+// Rows of S^T are keys; key i of an S tile t is key (i / 4) * 8 + 4 t + i % 4 of the step, so the 8
+// probabilities that a lane holds belong to 8 neighbouring keys: they are the B operand of the
+// second product as they stand, and its A operand is one 16 B load of a V row.  K and V go from
+// memory straight to registers.
+// ---------------------------------------------------------------------------------------------
+constexpr int kStep = 32;    // keys of a step
+constexpr float kSlack = 8;  // the running maximum may lag the true one by 2^8 (see below)
+
+struct Source {
+  const void *k_pool, *v_pool;
+  int n_pages, T, Tp, spp;  // spp: steps of a page
+};
+
+struct SharedArgs {
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  void* out;
+  int64_t o_sb, o_st, o_sh;
+  Source pre, own;
+  const int32_t* pre_pages;
+  int64_t pre_tokens;
+  const int32_t* tables;
+  int64_t table_st;
+  int width;
+  const int32_t* lengths;
+  const int32_t* new_lens;
+  int batch, rows, heads, group, causal;
+  float c;       // softmax_scale * log2(e)
+  int M;         // batch * rows * group
+  int pre_rb, pre_splits, pre_grid;  // row blocks, key splits and workgroups of the prefix
+  int own_rb, own_splits;            // row blocks of a sequence, key splits
+  int direct;    // one part only: workgroups write out themselves
+  float* part_o;   // [part][heads][M][128]
+  float2* part_ml; // [part][heads][M]
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+  typedef bf16x8 v8;
+  __device__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static constexpr uint32_t kInf = 0x7f80u;
+};
+template <>
+struct Mma<f16> {
+  typedef f16x8 v8;
+  __device__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static constexpr uint32_t kInf = 0x7c00u;
+};
+
+__device__ inline float over_keys_max(float x) {  // over the 4 lanes of a row
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ inline float over_keys_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// The page list of one work item, 64 entries in a vector register at a time.
+struct PageWalk {
+  const int32_t* list;
+  int n, base, ids;
+  __device__ void start(const int32_t* l, int count, int page) {
+    list = l;
+    n = count;
+    fill(page);
+  }
+  __device__ void fill(int page) {
+    base = page;
+    const int i = page + (int)(threadIdx.x & 63);
+    ids = i < n ? list[i] : -1;
+  }
+  __device__ int get(int page) {
+    if (page - base >= 64) fill(page);
+    return __builtin_amdgcn_readlane(ids, page - base);
+  }
+};
+
+template <typename T, int R>
+struct WaveState {
+  typename Mma<T>::v8 q[R][4];
+  f32x4 o[R][8];
+  float m[R], l[R];
+};
+
+// Steps [s0, s1) of a source's keys for one wave.  lim[r]: keys that the lane's row of tile r sees
+// (all of them where lim >= n_keys); every row sees the first `open` keys.
+template <typename T, int R>
+__device__ inline void walk(WaveState<T, R>& w, const Source& src, const int32_t* list, int n_list,
+                            int heads, int h, int64_t n_keys, int64_t open, const int64_t (&lim)[R],
+                            float c, int s0, int s1) {
+  typedef typename Mma<T>::v8 v8;
+  if (s0 >= s1) return;
+  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+  const int k_off = ((i16 >> 2) * 8 + (i16 & 3)) * kHeadDim + g * 8;
+  const int v_off = i16 * src.Tp + g * 8;
+  const T* kp = static_cast<const T*>(src.k_pool);
+  const T* vp = static_cast<const T*>(src.v_pool);
+  PageWalk pages;
+  int page = s0 / src.spp, in_page = s0 - page * src.spp;
+  pages.start(list, n_list, page);
+  int id = pages.get(page);
+  v8 kf[2][4];
+  auto load_k = [&](int id, int at) {
+    // a page that is not there is read as page 0 and masked
+    const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;
+    const T* p = kp + ((pid * heads + h) * src.Tp + at * kStep) * (int64_t)kHeadDim + k_off;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+        kf[t][st] = *reinterpret_cast<const v8*>(p + t * 4 * kHeadDim + st * 32);
+  };
+  load_k(id, in_page);
+  for (int s = s0; s < s1; ++s) {
+    const bool there = id >= 0 && id < src.n_pages;
+    const int64_t pid = there ? id : 0;
+    const T* vb = vp + (pid * heads + h) * kHeadDim * (int64_t)src.Tp + in_page * kStep;
+    v8 vf[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+      vf[d] = *reinterpret_cast<const v8*>(vb + d * 16 * src.Tp + v_off);
+    const int64_t key0 = (int64_t)page * src.T + in_page * kStep;
+    // keys of this step that exist: inside the page, inside the sequence
+    int64_t left = n_keys - key0;
+    const int in_tile = src.T - in_page * kStep;
+    if (left > in_tile) left = in_tile;
+    const int valid = there ? (left > kStep ? kStep : (int)left) : 0;
+    f32x4 sc[R][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) sc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < R; ++r) sc[r][t] = Mma<T>::mul(kf[t][st], w.q[r][st], sc[r][t]);
+    // the next step's keys load under this step's softmax and second product
+    if (s + 1 < s1) {
+      if (++in_page == src.spp) {
+        in_page = 0;
+        id = pages.get(++page);
+      }
+      load_k(id, in_page);
+    }
+    const bool partial = key0 + valid > open;  // some row may not see all of them
+    if (valid < kStep || partial) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int64_t seen = lim[r] - key0;
+        const int most = seen < valid ? (int)(seen < 0 ? 0 : seen) : valid;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (8 * g + 4 * t + i >= most) sc[r][t][i] = -INFINITY;
+      }
+      // what lies behind the last key is not multiplied, whatever the page holds there
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        u32x4 x = __builtin_bit_cast(u32x4, vf[d]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = 8 * g + 2 * e;
+          x[e] = key + 1 < valid ? x[e] : key < valid ? x[e] & 0xffffu : 0u;
+        }
+        vf[d] = __builtin_bit_cast(v8, x);
+      }
+    }
+    float top[R];
+    bool grow = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float t = sc[r][0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) t = fmaxf(t, sc[r][i >> 2][i & 3]);
+      top[r] = t * c;
+      grow |= top[r] > w.m[r] + kSlack;
+    }
+    // The maximum only has to keep exp2 in range, so it follows when some row of the wave is 2^8
+    // above it: most steps skip the reductions and the rescaling.
+    if (__any(grow)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float m = fmaxf(w.m[r], over_keys_max(top[r]));
+        const float a = m == w.m[r] ? 1.0f : __builtin_amdgcn_exp2f(w.m[r] - m);
+        w.m[r] = m;
+        w.l[r] *= a;
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[r][d][i] *= a;
+      }
+    }
+    v8 p[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float m = w.m[r] == -INFINITY ? 0.0f : w.m[r];
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(sc[r][i >> 2][i & 3] * c - m);
+        sum += e;
+        sc[r][i >> 2][i & 3] = e;
+        p[r][i] = (T)e;  // rounded to the pool's type for the matrix product; l sums it unrounded
+      }
+      w.l[r] += sum;
+    }
+    if (partial) {
+      // A key that some rows may not see yet can hold an infinity or a NaN, which 0 * v would
+      // spread to them: such values leave the product and are added to the rows that see them.
+      bool odd = false;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        u32x4 x = __builtin_bit_cast(u32x4, vf[d]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = Mma<T>::kInf, hi = lo << 16;
+          if ((x[e] & lo) == lo) x[e] &= 0xffff0000u, odd = true;
+          if ((x[e] & hi) == hi) x[e] &= 0xffffu, odd = true;
+        }
+        vf[d] = __builtin_bit_cast(v8, x);
+      }
+      if (__any(odd)) {
+#pragma unroll 1
+        for (int key = 0; key < valid; ++key) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float e = sc[r][0][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) e = (key & 7) == i ? sc[r][i >> 2][i & 3] : e;
+            e = __shfl(e, i16 + 16 * (key >> 3), 64);
+            const bool sees = key0 + key < lim[r];
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x = (float)vb[(16 * d + 4 * g + i) * (int64_t)src.Tp + key];
+                if (sees && !__builtin_isfinite(x)) w.o[r][d][i] += e * x;
+              }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int r = 0; r < R; ++r) w.o[r][d] = Mma<T>::mul(vf[d], p[r], w.o[r][d]);
+  }
+}
+
+// One work item: rows [m0, m1) of key head h against a share of a source's steps, by 4 waves: WR of
+// them side by side on 16 R rows each, 4 / WR behind one another along the keys.
+template <typename T, int R, int WR>
+__device__ inline void work_item(const SharedArgs& a, const Source& src, const int32_t* list,
+                                 int n_list, int h, int m0, int m1, int64_t n_keys, int64_t open,
+                                 int64_t first_lim, int n_split, int split, int part, float* lds) {
+  constexpr int WK = 4 / WR;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave % WR, wk = wave / WR;
+  const int i16 = lane & 15, g = lane >> 4;
+  WaveState<T, R> w;
+  int64_t lim[R];
+  int row_of[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int m = m0 + (wr * R + r) * 16 + i16;
+    row_of[r] = m < m1 ? m : -1;
+    const int mm = m < m1 ? m : m0;
+    const int gh = mm % a.group, bl = mm / a.group, l = bl % a.rows, b = bl / a.rows;
+    // first_lim: own keys that the sequence's row 0 sees, one more for each next row (causal)
+    lim[r] = a.causal && first_lim != INT64_MAX ? first_lim + l : n_keys;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
+                 (int64_t)(h * a.group + gh) * a.q_sh + g * 8;
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+      w.q[r][st] = *reinterpret_cast<const typename Mma<T>::v8*>(q + st * 32);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) w.o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w.m[r] = -INFINITY;
+    w.l[r] = 0.0f;
+  }
+  // steps of the item: whole pages, then what the last page holds
+  const int64_t full = n_keys / src.T;
+  const int rest = (int)(n_keys - full * src.T);
+  const int n_steps = (int)(full * src.spp) + (rest + kStep - 1) / kStep;
+  const int share = n_split * WK, mine = split * WK + wk;
+  const int s0 = (int)((int64_t)n_steps * mine / share), s1 = (int)((int64_t)n_steps * (mine + 1) / share);
+  walk<T, R>(w, src, list, n_list, a.heads, h, n_keys, open, lim, a.c, s0, s1);
+#pragma unroll
+  for (int r = 0; r < R; ++r) w.l[r] = over_keys_sum(w.l[r]);
+  // waves along the keys join in halves through LDS
+  if constexpr (WK > 1) {
+    constexpr int kPer = R * 34 * 64;  // floats of a wave's state: 32 outputs, m and l a lane and tile
+#pragma unroll
+    for (int half = WK / 2; half > 0; half >>= 1) {
+      float* at = lds + ((wk % half) * WR + wr) * kPer + lane;
+      if (wk >= half && wk < 2 * half) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) at[(r * 34 + e) * 64] = w.o[r][e >> 2][e & 3];
+          at[(r * 34 + 32) * 64] = w.m[r];
+          at[(r * 34 + 33) * 64] = w.l[r];
+        }
+      }
+      __syncthreads();
+      if (wk < half) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float m2 = at[(r * 34 + 32) * 64], l2 = at[(r * 34 + 33) * 64];
+          const float m = fmaxf(w.m[r], m2), ms = m == -INFINITY ? 0.0f : m;
+          const float x = __builtin_amdgcn_exp2f(w.m[r] - ms), y = __builtin_amdgcn_exp2f(m2 - ms);
+          w.m[r] = m;
+          w.l[r] = w.l[r] * x + l2 * y;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            w.o[r][e >> 2][e & 3] = w.o[r][e >> 2][e & 3] * x + at[(r * 34 + e) * 64] * y;
+        }
+      }
+      __syncthreads();
+    }
+    if (wk > 0) return;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int m = row_of[r];
+    if (m < 0) continue;
+    if (a.direct) {
+      const int gh = m % a.group, bl = m / a.group, l = bl % a.rows, b = bl / a.rows;
+      int fresh = a.rows;
+      if (a.new_lens != nullptr) fresh = a.new_lens[b];
+      const float inv = l < fresh && w.l[r] != 0.0f ? 1.0f / w.l[r] : 0.0f;
+      T* o = static_cast<T*>(a.out) + b * a.o_sb + l * a.o_st + (int64_t)(h * a.group + gh) * a.o_sh + g * 4;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = inv != 0.0f ? (T)(w.o[r][d][i] * inv) : (T)0.0f;
+        *reinterpret_cast<t4*>(o + 16 * d) = x;
+      }
+    } else {
+      const int64_t at = ((int64_t)part * a.heads + h) * a.M + m;
+      float* o = a.part_o + at * kHeadDim + g * 4;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = w.o[r][d];
+      if (g == 0) a.part_ml[at] = float2{w.m[r], w.l[r]};
+    }
+  }
+}
+
+// The prefix's work items first, dealt so that the row blocks of one (key head, split) run on one
+// XCD and share its L2; then every sequence's own pages.
+template <typename T, int RP, int WRP, int RO, int WRO>
+__global__ __launch_bounds__(256) void attend_shared_kernel(SharedArgs a) {
+  constexpr int kP = WRP < 4 ? 2 * RP * 34 * 64 : 0, kO = WRO < 4 ? 2 * RO * 34 * 64 : 0;
+  __shared__ float lds[(kP > kO ? kP : kO) > 0 ? (kP > kO ? kP : kO) : 1];
+  int bid = blockIdx.x;
+  if (bid < a.pre_grid) {
+    const int idx = bid >> 3, pair = (idx / a.pre_rb) * 8 + (bid & 7), rb = idx % a.pre_rb;
+    if (pair >= a.heads * a.pre_splits) return;
+    const int h = pair % a.heads, split = pair / a.heads;
+    const int m0 = rb * 16 * RP * WRP;
+    const int m1 = m0 + 16 * RP * WRP < a.M ? m0 + 16 * RP * WRP : a.M;
+    const int64_t n_list = (a.pre_tokens + a.pre.T - 1) / a.pre.T;
+    work_item<T, RP, WRP>(a, a.pre, a.pre_pages, (int)n_list, h, m0, m1, a.pre_tokens, a.pre_tokens,
+                          INT64_MAX, a.pre_splits, split, split, lds);
+    return;
+  }
+  bid -= a.pre_grid;
+  const int split = bid % a.own_splits;
+  bid /= a.own_splits;
+  const int rb = bid % a.own_rb;
+  bid /= a.own_rb;
+  const int h = bid % a.heads, b = bid / a.heads;
+  const int per = a.rows * a.group;
+  const int m0 = b * per + rb * 16 * RO * WRO;
+  const int m1 = m0 + 16 * RO * WRO < (b + 1) * per ? m0 + 16 * RO * WRO : (b + 1) * per;
+  int fresh = a.rows;
+  if (a.new_lens != nullptr) {
+    fresh = a.new_lens[b];
+    fresh = fresh < 0 ? 0 : fresh > a.rows ? a.rows : fresh;
+  }
+  int64_t n_keys = a.lengths[b];
+  const int64_t cap = (int64_t)a.width * a.own.T;
+  // rows of a causal sequence: row l sees lengths - fresh + l + 1 keys, whatever the table holds
+  int64_t first_lim = n_keys - fresh + 1;
+  n_keys = n_keys < 0 ? 0 : n_keys > cap ? cap : n_keys;
+  const int64_t open = a.causal ? first_lim + (m0 - b * per) / a.group : n_keys;
+  work_item<T, RO, WRO>(a, a.own, a.tables + b * a.table_st, a.width, h, m0, m1, n_keys, open, first_lim,
+                        a.own_splits, split, a.pre_splits + split, lds);
+}
+
+// One wave per (row, key head): the parts' weights, then their outputs, a lane two channels.
+template <typename T>
+__global__ __launch_bounds__(256) void merge_kernel(SharedArgs a, int n_parts) {
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (unit >= (int64_t)a.heads * a.M) return;
+  const int h = (int)(unit % a.heads), m = (int)(unit / a.heads);
+  const int gh = m % a.group, bl = m / a.group, l = bl % a.rows, b = bl / a.rows;
+  int fresh = a.rows;
+  if (a.new_lens != nullptr) fresh = a.new_lens[b];
+  const int64_t at = (int64_t)h * a.M + m, step = (int64_t)a.heads * a.M;
+  float x = 0.0f, y = 0.0f, total = 0.0f;
+  if (l < fresh) {
+    float top = -INFINITY;
+    for (int p = lane; p < n_parts; p += 64) top = fmaxf(top, a.part_ml[at + p * step].x);
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+    if (top == -INFINITY) top = 0.0f;
+    for (int p = 0; p < n_parts; ++p) {
+      const float2 ml = a.part_ml[at + p * step];
+      const float s = __builtin_amdgcn_exp2f(ml.x - top);
+      const float2 o = *reinterpret_cast<const float2*>(a.part_o + (at + p * step) * kHeadDim + 2 * lane);
+      total += s * ml.y;
+      x += s * o.x;
+      y += s * o.y;
+    }
+  }
+  const bool any = total != 0.0f;  // a row that sees no key is zero (NaN sums are not zero)
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  t2 r;
+  r[0] = any ? (T)(x / total) : (T)0.0f;
+  r[1] = any ? (T)(y / total) : (T)0.0f;
+  T* o = static_cast<T*>(a.out) + b * a.o_sb + l * a.o_st + (int64_t)(h * a.group + gh) * a.o_sh;
+  *reinterpret_cast<t2*>(o + 2 * lane) = r;
+}
+
+// ---------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------
+bool half_dtype(int t) { return t == SKV_BF16 || t == SKV_F16; }
+
+bool view_ok(const void* p, int64_t sb, int64_t st, int64_t sh) {
+  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb >= 0 && st >= 0 && sh >= 0 &&
+         sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0;
+}
+
+bool pool_ok(const void* k, const void* v) {
+  return k && v && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+}
+
+int launched(const char* fn) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return SKV_OK;
+  set_error("%s: launch failed: %s", fn, hipGetErrorString(e));
+  return SKV_E_LAUNCH;
+}
+
+int common_errors(const char* fn, int dtype, int head_dim, int batch, int rows, int q_heads,
+                  int kv_heads, int n_pages, int page_tokens, const int32_t* tables,
+                  int64_t table_stride, int table_width, const int32_t* lengths, bool q_needed) {
+  if (head_dim != kHeadDim) {
+    set_error("%s: head_dim=%d unsupported (built for %d)", fn, head_dim, kHeadDim);
+    return SKV_E_UNSUPPORTED;
+  }
+  if (!half_dtype(dtype)) {
+    set_error("%s: dtype %d unsupported (bf16 or f16)", fn, dtype);
+    return SKV_E_UNSUPPORTED;
+  }
+  if (batch < 0 || rows < 0 || kv_heads <= 0 || (q_needed && (q_heads <= 0 || q_heads % kv_heads))) {
+    set_error("%s: bad sizes (batch=%d rows=%d, %d query heads over %d key heads)", fn, batch, rows,
+              q_heads, kv_heads);
+    return SKV_E_ARG;
+  }
+  if (n_pages <= 0 || page_tokens <= 0 || page_tokens > (1 << 24)) {
+    set_error("%s: bad pool (%d pages of %d tokens)", fn, n_pages, page_tokens);
+    return SKV_E_ARG;
+  }
+  if (table_width < 0 || (table_width > 0 && (!tables || table_stride < 0)) || !lengths ||
+      (int64_t)table_width * page_tokens >= ((int64_t)1 << 31)) {
+    set_error("%s: bad page tables (width=%d) or no lengths", fn, table_width);
+    return SKV_E_ARG;
+  }
+  return SKV_OK;
+}
+
+// The launch of an attention: row tiles and waves of both kinds of work item, and the splits.
+struct SharedPlan {
+  int pre_kind, own_kind;  // 0: 16 rows, waves along the keys; 1: 64 rows; 2: 128 rows
+  int pre_rb, pre_splits, pre_grid, own_rb, own_splits, own_grid, parts;
+  int64_t bytes;
+};
+
+constexpr int kKindRows[3] = {16, 64, 128};
+constexpr int kKindWK[3] = {4, 2, 1};  // waves along the keys
+
+int kind_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 64 ? 1 : 2; }
+
+int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) {
+  const int group = d->q_heads / d->kv_heads;
+  const int64_t M = (int64_t)d->batch * d->rows * group, per = (int64_t)d->rows * group;
+  if (M * d->kv_heads >= ((int64_t)1 << 30)) {
+    set_error("%s: too many query rows (batch=%d rows=%d heads=%d)", fn, d->batch, d->rows, d->q_heads);
+    return SKV_E_ARG;
+  }
+  *p = SharedPlan{};
+  const bool pre = d->prefix_tokens > 0, own = d->table_width > 0;
+  p->pre_kind = kind_of(M);
+  p->own_kind = kind_of(per);
+  if (!pre) p->pre_kind = p->own_kind;
+  const int64_t cu = cu_count();
+  // steps of 32 keys that one wave would take, over all work items
+  const int64_t pre_steps = pre ? (d->prefix_tokens / d->prefix_page_tokens) *
+                                          ((d->prefix_page_tokens + kStep - 1) / kStep) +
+                                      (d->prefix_tokens % d->prefix_page_tokens + kStep - 1) / kStep
+                                : 0;
+  const int64_t own_steps = own ? (int64_t)d->table_width * ((d->page_tokens + kStep - 1) / kStep) : 0;
+  p->pre_rb = pre ? (int)((M + kKindRows[p->pre_kind] - 1) / kKindRows[p->pre_kind]) : 0;
+  p->own_rb = own ? (int)((per + kKindRows[p->own_kind] - 1) / kKindRows[p->own_kind]) : 0;
+  const int64_t pre_items = (int64_t)p->pre_rb * d->kv_heads;
+  const int64_t own_items = (int64_t)p->own_rb * d->kv_heads * d->batch;
+  const int64_t wave_steps = pre_items * ((pre_steps + kKindWK[p->pre_kind] - 1) / kKindWK[p->pre_kind]) +
+                             own_items * ((own_steps + kKindWK[p->own_kind] - 1) / kKindWK[p->own_kind]);
+  int64_t share = (wave_steps + 2 * cu - 1) / (2 * cu);  // steps of a wave with two workgroups a CU
+  if (share < 4) share = 4;
+  auto splits = [&](int64_t steps, int kind) -> int {
+    const int64_t s = (steps + share * kKindWK[kind] - 1) / (share * kKindWK[kind]);
+    return (int)(s < 1 ? 1 : s > 1024 ? 1024 : s);
+  };
+  p->pre_splits = pre ? splits(pre_steps, p->pre_kind) : 0;
+  p->own_splits = own ? splits(own_steps, p->own_kind) : 0;
+  p->parts = p->pre_splits + p->own_splits;
+  const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits;
+  const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, own_grid = own_items * p->own_splits;
+  if (pre_grid + own_grid >= ((int64_t)1 << 31)) {
+    set_error("%s: too many work items", fn);
+    return SKV_E_ARG;
+  }
+  p->pre_grid = (int)pre_grid;
+  p->own_grid = (int)own_grid;
+  p->bytes = p->parts > 1 ? (int64_t)p->parts * d->kv_heads * M * (kHeadDim * 4 + 8) : 0;
+  return SKV_OK;
+}
+
+int check_shared(const char* fn, const skv_attend_shared_desc* d) {
+  clear_error();
+  if (!d) {
+    set_error("%s: null descriptor", fn);
+    return SKV_E_ARG;
+  }
+  const int st = common_errors(fn, d->dtype, d->head_dim, d->batch, d->rows, d->q_heads, d->kv_heads,
+                               d->n_pages, d->page_tokens, d->tables, d->table_stride, d->table_width,
+                               d->lengths, true);
+  if (st != SKV_OK) return st;
+  if (!view_ok(d->q, d->q_sb, d->q_st, d->q_sh) || !view_ok(d->out, d->out_sb, d->out_st, d->out_sh)) {
+    set_error("%s: q and out must be 16-byte aligned with non-negative strides that are multiples of "
+              "8 elements", fn);
+    return SKV_E_ARG;
+  }
+  if (!pool_ok(d->k_pool, d->v_pool)) {
+    set_error("%s: pools must be 16-byte aligned", fn);
+    return SKV_E_ARG;
+  }
+  if (d->prefix_tokens < 0 ||
+      (d->prefix_tokens > 0 &&
+       (!pool_ok(d->prefix_k_pool, d->prefix_v_pool) || !d->prefix_pages || d->prefix_n_pages <= 0 ||
+        d->prefix_page_tokens <= 0 || d->prefix_page_tokens > (1 << 24) ||
+        d->prefix_tokens >= ((int64_t)1 << 31)))) {
+    set_error("%s: bad prefix (%lld tokens in pages of %d)", fn, (long long)d->prefix_tokens,
+              d->prefix_page_tokens);
+    return SKV_E_ARG;
+  }
+  if (!(d->softmax_scale > 0.0f) || d->softmax_scale > 3.0e38f) {
+    set_error("%s: softmax_scale must be positive and finite", fn);
+    return SKV_E_ARG;
+  }
+  return SKV_OK;
+}
+
+template <typename T>
+void launch_shared(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.pre_grid + p.own_grid)), block(256);
+#define SKV_KINDS(P, O, RP, WRP, RO, WRO)                                                        \
+  if (p.pre_kind == P && p.own_kind == O) {                                                      \
+    hipLaunchKernelGGL((attend_shared_kernel<T, RP, WRP, RO, WRO>), grid, block, 0, s, a);       \
+    return;                                                                                      \
+  }
+  SKV_KINDS(0, 0, 1, 1, 1, 1)
+  SKV_KINDS(1, 0, 2, 2, 1, 1)
+  SKV_KINDS(1, 1, 2, 2, 2, 2)
+  SKV_KINDS(2, 0, 2, 4, 1, 1)
+  SKV_KINDS(2, 1, 2, 4, 2, 2)
+  SKV_KINDS(2, 2, 2, 4, 2, 4)
+#undef SKV_KINDS
+}
+
+}  // namespace
+
+}  // namespace skv
+
+using namespace skv;
+
+extern "C" int skv_append_pages(const skv_append_pages_desc* d, skv_stream_t stream) {
+  const char* fn = "skv_append_pages";
+  clear_error();
+  if (!d) {
+    set_error("%s: null descriptor", fn);
+    return SKV_E_ARG;
+  }
+  int st = common_errors(fn, d->dtype, d->head_dim, d->batch, d->rows, d->q_heads, d->kv_heads, d->n_pages,
+                         d->page_tokens, d->tables, d->table_stride, d->table_width, d->lengths, false);
+  if (st != SKV_OK) return st;
+  const bool q = d->q_heads > 0;
+  if (d->q_heads < 0 || !view_ok(d->k, d->k_sb, d->k_st, d->k_sh) || !view_ok(d->v, d->v_sb, d->v_st, d->v_sh) ||
+      (q && (!view_ok(d->q, d->q_sb, d->q_st, d->q_sh) || !view_ok(d->q_out, d->out_sb, d->out_st, d->out_sh)))) {
+    set_error("%s: k, v, q and q_out must be 16-byte aligned with non-negative strides that are "
+              "multiples of 8 elements", fn);
+    return SKV_E_ARG;
+  }
+  if (!pool_ok(d->k_pool, d->v_pool)) {
+    set_error("%s: pools must be 16-byte aligned", fn);
+    return SKV_E_ARG;
+  }
+  if (d->half < 0 || d->half > kHeadDim / 2 || d->half % 8 || (d->half > 0) != (d->cos != nullptr) ||
+      (d->cos == nullptr) != (d->sin == nullptr)) {
+    set_error("%s: the rotation takes cos and sin of 8, 16 .. 64 columns, or neither", fn);
+    return SKV_E_ARG;
+  }
+  if (d->half && (d->table_rows <= 0 || d->cos_stride < d->half || d->cos_stride % 4 ||
+                  reinterpret_cast<uintptr_t>(d->cos) % 16 || reinterpret_cast<uintptr_t>(d->sin) % 16)) {
+    set_error("%s: cos / sin need rows, 16-byte aligned pointers and a row stride that is a "
+              "multiple of 4 and holds the columns", fn);
+    return SKV_E_ARG;
+  }
+  const skv_head_norm* norms[2] = {&d->norm_q, &d->norm_k};
+  for (const skv_head_norm* n : norms) {
+    if (n->norm && (!(n->eps >= 0.0f) ||
+                    (n->weight && (reinterpret_cast<uintptr_t>(n->weight) % 16 ||
+                                   (n->weight_dtype != SKV_F32 && !half_dtype(n->weight_dtype)))))) {
+      set_error("%s: norms need eps >= 0 and 16-byte aligned f32, bf16 or f16 weights", fn);
+      return SKV_E_ARG;
+    }
+  }
+  AppendPagesArgs a{};
+  a.pg.tables = d->tables, a.pg.table_st = d->table_stride, a.pg.width = d->table_width;
+  a.pg.n_pages = d->n_pages, a.pg.T = d->page_tokens, a.pg.Tp = padded_tokens(d->page_tokens);
+  a.pg.heads = d->kv_heads, a.pg.lengths = d->lengths, a.pg.new_lens = d->new_lens;
+  a.q = d->q, a.q_sb = d->q_sb, a.q_st = d->q_st, a.q_sh = d->q_sh;
+  a.k = d->k, a.k_sb = d->k_sb, a.k_st = d->k_st, a.k_sh = d->k_sh;
+  a.v = d->v, a.v_sb = d->v_sb, a.v_st = d->v_st, a.v_sh = d->v_sh;
+  a.q_out = d->q_out, a.o_sb = d->out_sb, a.o_st = d->out_st, a.o_sh = d->out_sh;
+  a.k_pool = d->k_pool, a.v_pool = d->v_pool;
+  a.wq = d->norm_q.norm ? d->norm_q.weight : nullptr, a.wq_dtype = d->norm_q.weight_dtype;
+  a.wk = d->norm_k.norm ? d->norm_k.weight : nullptr, a.wk_dtype = d->norm_k.weight_dtype;
+  a.norm_q = d->norm_q.norm != 0, a.norm_k = d->norm_k.norm != 0;
+  a.eps_q = d->norm_q.eps, a.eps_k = d->norm_k.eps;
+  a.q_heads = d->q_heads, a.q_blocks = (d->q_heads + kHeadBlock - 1) / kHeadBlock;
+  a.k_blocks = (d->kv_heads + kHeadBlock - 1) / kHeadBlock;
+  a.cos = d->cos, a.sin = d->sin, a.tab_st = d->cos_stride, a.tab_rows = d->table_rows;
+  a.pos = d->positions, a.pos_sb = d->pos_sb, a.pos_st = d->pos_st, a.pos0 = d->position0;
+  a.pos64 = d->pos_is_int64, a.half = d->half, a.batch = d->batch, a.rows = d->rows;
+  const int64_t tokens = (int64_t)d->batch * d->rows;
+  if (tokens == 0) return SKV_OK;
+  // A tile of a page (through LDS, 16 B stores) pays off once a sequence brings several tokens;
+  // fewer go to their places one by one.
+  int64_t v_groups;
+  if (d->rows >= 8) {
+    const int64_t per_page = (d->page_tokens + kTile - 1) / kTile, ends = (d->rows + d->page_tokens - 2) / d->page_tokens;
+    const int64_t by_tile = (d->rows - 1) / kTile + 2 + ends, by_page = (ends + 1) * per_page;
+    a.v_tiles = (int)(by_tile < by_page ? by_tile : by_page);
+    v_groups = (int64_t)d->batch * d->kv_heads * a.v_tiles;
+  } else {
+    v_groups = (tokens * d->kv_heads + 3) / 4;
+  }
+  const int64_t units = tokens * (a.q_blocks + a.k_blocks), groups = (units + 15) / 16;
+  if (units >= ((int64_t)1 << 30) || v_groups >= ((int64_t)1 << 30) ||
+      tokens * d->kv_heads >= ((int64_t)1 << 30)) {
+    set_error("%s: too many rows (batch=%d rows=%d)", fn, d->batch, d->rows);
+    return SKV_E_ARG;
+  }
+  a.n_units_q = (int)(tokens * a.q_blocks);
+  a.n_units = (int)units;
+  a.n_unit_groups = (int)groups;
+  const dim3 grid((unsigned)(groups + v_groups)), block(256);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->dtype == SKV_BF16) {
+    if (d->interleaved) hipLaunchKernelGGL((append_pages_kernel<bf16, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((append_pages_kernel<bf16, false>), grid, block, 0, s, a);
+  } else {
+    if (d->interleaved) hipLaunchKernelGGL((append_pages_kernel<f16, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((append_pages_kernel<f16, false>), grid, block, 0, s, a);
+  }
+  return launched(fn);
+}
+
+extern "C" int skv_attend_shared_workspace(const skv_attend_shared_desc* d, int64_t* bytes) {
+  const char* fn = "skv_attend_shared_workspace";
+  int st = check_shared(fn, d);
+  if (st != SKV_OK) return st;
+  if (!bytes) {
+    set_error("%s: null result", fn);
+    return SKV_E_ARG;
+  }
+  SharedPlan p;
+  st = plan_shared(fn, d, &p);
+  if (st == SKV_OK) *bytes = p.bytes;
+  return st;
+}
+
+extern "C" int skv_attend_shared(const skv_attend_shared_desc* d, skv_stream_t stream) {
+  const char* fn = "skv_attend_shared";
+  int st = check_shared(fn, d);
+  if (st != SKV_OK) return st;
+  SharedPlan p;
+  st = plan_shared(fn, d, &p);
+  if (st != SKV_OK) return st;
+  if (d->batch == 0 || d->rows == 0) return SKV_OK;
+  if (p.bytes > 0 && (!d->workspace || d->workspace_bytes < p.bytes ||
+                      reinterpret_cast<uintptr_t>(d->workspace) % 16)) {
+    set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)p.bytes);
+    return SKV_E_ARG;
+  }
+  SharedArgs a{};
+  a.q = d->q, a.q_sb = d->q_sb, a.q_st = d->q_st, a.q_sh = d->q_sh;
+  a.out = d->out, a.o_sb = d->out_sb, a.o_st = d->out_st, a.o_sh = d->out_sh;
+  a.own = Source{d->k_pool, d->v_pool, d->n_pages, d->page_tokens, padded_tokens(d->page_tokens),
+                 (d->page_tokens + kStep - 1) / kStep};
+  if (d->prefix_tokens > 0)
+    a.pre = Source{d->prefix_k_pool, d->prefix_v_pool, d->prefix_n_pages, d->prefix_page_tokens,
+                   padded_tokens(d->prefix_page_tokens), (d->prefix_page_tokens + kStep - 1) / kStep};
+  a.pre_pages = d->prefix_pages, a.pre_tokens = d->prefix_tokens;
+  a.tables = d->tables, a.table_st = d->table_stride, a.width = d->table_width;
+  a.lengths = d->lengths, a.new_lens = d->new_lens;
+  a.batch = d->batch, a.rows = d->rows, a.heads = d->kv_heads, a.group = d->q_heads / d->kv_heads;
+  a.causal = d->causal != 0, a.c = d->softmax_scale * 1.44269504088896340736f;
+  a.M = d->batch * d->rows * a.group;
+  a.pre_rb = p.pre_rb, a.pre_splits = p.pre_splits, a.pre_grid = p.pre_grid;
+  a.own_rb = p.own_rb, a.own_splits = p.own_splits;
+  a.direct = p.parts == 1;
+  a.part_o = static_cast<float*>(d->workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)p.parts * a.heads * a.M * kHeadDim);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.pre_grid + p.own_grid > 0) {
+    if (d->dtype == SKV_BF16) launch_shared<bf16>(a, p, s);
+    else launch_shared<f16>(a, p, s);
+    st = launched(fn);
+    if (st != SKV_OK || a.direct) return st;
+  }
+  const dim3 grid((unsigned)(((int64_t)a.heads * a.M + 3) / 4)), block(256);
+  if (d->dtype == SKV_BF16) hipLaunchKernelGGL(merge_kernel<bf16>, grid, block, 0, s, a, p.parts);
+  else hipLaunchKernelGGL(merge_kernel<f16>, grid, block, 0, s, a, p.parts);
+  return launched(fn);
+}
