@@ -216,18 +216,20 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
 // and its unnormalised fp32 output, which merge_kernel joins:
 //   out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p,  m = max m_p.
 //
-// A wave works on 16 R rows and 32 keys a step: S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs.
-// Rows of S^T are keys; key i of an S tile t is key (i / 4) * 8 + 4 t + i % 4 of the step, so the 8
-// probabilities that a lane holds belong to 8 neighbouring keys: they are the B operand of the
-// second product as they stand, and its A operand is one 16 B load of a V row.  K and V go from
-// memory straight to registers.
+// S^T = K Q^T and O^T = V^T P^T, so a lane holds one row's scores.  The rows of S^T are keys in an
+// order that makes the probabilities a lane holds those of neighbouring keys: they are the second
+// product's B operand as they stand, and its A operand is 16 B pieces of V rows.
+//
+// Few rows (at most 16 of a key head) stream: each of 4 waves takes its own share of the keys, K and
+// V straight from memory to registers, bound by bytes.  More rows share: 4 waves of 32 rows read
+// tiles of 64 keys that the workgroup stages in LDS, bound by the matrix cores.
 // ---------------------------------------------------------------------------------------------
-constexpr int kStep = 32;    // keys of a step
+constexpr int kStep = 32;    // keys of a streaming step
 constexpr float kSlack = 8;  // the running maximum may lag the true one by 2^8 (see below)
 
 struct Source {
   const void *k_pool, *v_pool;
-  int n_pages, T, Tp, spp;  // spp: steps of a page
+  int n_pages, T, Tp;
 };
 
 struct SharedArgs {
@@ -253,6 +255,16 @@ struct SharedArgs {
   float2* part_ml; // [part][heads][M]
 };
 
+// One work item: rows [m0, m1) of key head h against share `split` of `n_split` of a source's keys.
+struct Item {
+  const int32_t* list;  // page numbers
+  int n_list, h, m0, m1, n_split, split, part;
+  int64_t n_keys;     // keys that some row sees
+  int64_t open;       // keys that every row sees
+  int64_t first_lim;  // keys that row 0 of the sequence sees (causal; each next row one more)
+  bool causal;
+};
+
 template <typename T>
 struct Mma;
 template <>
@@ -260,6 +272,9 @@ struct Mma<bf16> {
   typedef bf16x8 v8;
   __device__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ static f32x16 mul(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static constexpr uint32_t kInf = 0x7f80u;
 };
@@ -269,19 +284,57 @@ struct Mma<f16> {
   __device__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
+  __device__ static f32x16 mul(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
   static constexpr uint32_t kInf = 0x7c00u;
 };
 
-__device__ inline float over_keys_max(float x) {  // over the 4 lanes of a row
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+__device__ inline float over_groups_max(float x, int first) {  // over the lanes of a row
+  for (int s = first; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s, 64));
+  return x;
 }
-__device__ inline float over_keys_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+__device__ inline float over_groups_sum(float x, int first) {
+  for (int s = first; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
+  return x;
 }
 
-// The page list of one work item, 64 entries in a vector register at a time.
+// 8 neighbouring values of a V row starting at key `k0`: those at or behind `valid` become zero, so
+// that what a page holds there is not multiplied.
+template <typename V8>
+__device__ inline V8 drop_behind(V8 v, int k0, int valid) {
+  u32x4 x = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    x[e] = k0 + 2 * e + 1 < valid ? x[e] : k0 + 2 * e < valid ? x[e] & 0xffffu : 0u;
+  return __builtin_bit_cast(V8, x);
+}
+
+// Infinities and NaN of a V piece become zero; returns whether there were any.
+template <typename T>
+__device__ inline bool drop_odd(typename Mma<T>::v8& v) {
+  u32x4 x = __builtin_bit_cast(u32x4, v);
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = Mma<T>::kInf, hi = lo << 16;
+    if ((x[e] & lo) == lo) x[e] &= 0xffff0000u, odd = true;
+    if ((x[e] & hi) == hi) x[e] &= 0xffffu, odd = true;
+  }
+  v = __builtin_bit_cast(typename Mma<T>::v8, x);
+  return odd;
+}
+
+// Element i of a piece, i known at run time only.
+template <typename T>
+__device__ inline float pick(typename Mma<T>::v8 v, int i) {
+  const u32x4 x = __builtin_bit_cast(u32x4, v);
+  const uint32_t w = i < 4 ? (i < 2 ? x[0] : x[1]) : (i < 6 ? x[2] : x[3]);
+  const uint16_t bits = (uint16_t)(i & 1 ? w >> 16 : w);
+  return (float)__builtin_bit_cast(T, bits);
+}
+
+// A work item's page list, 64 entries in a vector register at a time.
 struct PageWalk {
   const int32_t* list;
   int n, base, ids;
@@ -301,322 +354,451 @@ struct PageWalk {
   }
 };
 
-template <typename T, int R>
-struct WaveState {
-  typename Mma<T>::v8 q[R][4];
-  f32x4 o[R][8];
-  float m[R], l[R];
-};
+// The steps of `step` keys that n_keys take: whole pages, then what the last page holds.
+__device__ inline int steps_of(const Source& src, int64_t n_keys, int step, int per_page) {
+  const int64_t full = n_keys / src.T;
+  return (int)(full * per_page) + ((int)(n_keys - full * src.T) + step - 1) / step;
+}
 
-// Steps [s0, s1) of a source's keys for one wave.  lim[r]: keys that the lane's row of tile r sees
-// (all of them where lim >= n_keys); every row sees the first `open` keys.
-template <typename T, int R>
-__device__ inline void walk(WaveState<T, R>& w, const Source& src, const int32_t* list, int n_list,
-                            int heads, int h, int64_t n_keys, int64_t open, const int64_t (&lim)[R],
-                            float c, int s0, int s1) {
+__device__ inline void row_of(const SharedArgs& a, int m, int& b, int& l, int& gh) {
+  gh = m % a.group;
+  const int bl = m / a.group;
+  l = bl % a.rows;
+  b = bl / a.rows;
+}
+
+__device__ inline int fresh_rows(const SharedArgs& a, int b) {
+  if (a.new_lens == nullptr) return a.rows;
+  const int n = a.new_lens[b];
+  return n < 0 ? 0 : n > a.rows ? a.rows : n;
+}
+
+// Four neighbouring output channels d0 .. d0 + 3 of row m, or of its part.
+template <typename T>
+__device__ inline void put4(const SharedArgs& a, const Item& it, int m, int d0, f32x4 o, float inv, T* dst) {
+  if (a.direct) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = inv != 0.0f ? (T)(o[i] * inv) : (T)0.0f;
+    *reinterpret_cast<t4*>(dst + d0) = x;
+  } else {
+    const int64_t at = ((int64_t)it.part * a.heads + it.h) * a.M + m;
+    *reinterpret_cast<f32x4*>(a.part_o + at * kHeadDim + d0) = o;
+  }
+}
+
+// 1 / l of a row that is a new token and sees a key, else 0; and where its output goes.
+template <typename T>
+__device__ inline float row_out(const SharedArgs& a, const Item& it, int m, float mx, float l, bool first, T** dst) {
+  if (!a.direct) {
+    if (first) a.part_ml[((int64_t)it.part * a.heads + it.h) * a.M + m] = float2{mx, l};
+    return 0.0f;
+  }
+  int b, row, gh;
+  row_of(a, m, b, row, gh);
+  *dst = static_cast<T*>(a.out) + b * a.o_sb + row * a.o_st + (int64_t)(it.h * a.group + gh) * a.o_sh;
+  return row < fresh_rows(a, b) && l != 0.0f ? 1.0f / l : 0.0f;
+}
+
+// OWN: a sequence's own keys, which some rows may not see yet (the prefix is seen by all).
+
+// ---- at most 16 rows: a wave streams its own keys, 32 a step, on 16x16x32 MFMAs ----------------
+// Row i of S tile t is key (i / 4) * 8 + 4 t + i % 4 of the step; lane (n, g) holds row n's keys
+// 8 g .. 8 g + 7.
+template <typename T, bool OWN>
+__device__ inline void stream_item(const SharedArgs& a, const Source& src, const Item& it, float* lds) {
   typedef typename Mma<T>::v8 v8;
-  if (s0 >= s1) return;
-  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
-  const int k_off = ((i16 >> 2) * 8 + (i16 & 3)) * kHeadDim + g * 8;
-  const int v_off = i16 * src.Tp + g * 8;
-  const T* kp = static_cast<const T*>(src.k_pool);
-  const T* vp = static_cast<const T*>(src.v_pool);
-  PageWalk pages;
-  int page = s0 / src.spp, in_page = s0 - page * src.spp;
-  pages.start(list, n_list, page);
-  int id = pages.get(page);
-  v8 kf[2][4];
-  auto load_k = [&](int id, int at) {
-    // a page that is not there is read as page 0 and masked
-    const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;
-    const T* p = kp + ((pid * heads + h) * src.Tp + at * kStep) * (int64_t)kHeadDim + k_off;
+  const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int m = it.m0 + n;
+  int b, l, gh;
+  row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
+  const int64_t lim = OWN && it.causal ? it.first_lim + l : it.n_keys;
+  v8 q[4];
+  {
+    const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
+                 (int64_t)(it.h * a.group + gh) * a.q_sh + g * 8;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int st = 0; st < 4; ++st) q[st] = *reinterpret_cast<const v8*>(p + st * 32);
+  }
+  f32x4 o[8];
 #pragma unroll
-      for (int st = 0; st < 4; ++st)
-        kf[t][st] = *reinterpret_cast<const v8*>(p + t * 4 * kHeadDim + st * 32);
-  };
-  load_k(id, in_page);
-  for (int s = s0; s < s1; ++s) {
-    const bool there = id >= 0 && id < src.n_pages;
-    const int64_t pid = there ? id : 0;
-    const T* vb = vp + (pid * heads + h) * kHeadDim * (int64_t)src.Tp + in_page * kStep;
-    v8 vf[8];
-#pragma unroll
-    for (int d = 0; d < 8; ++d)
-      vf[d] = *reinterpret_cast<const v8*>(vb + d * 16 * src.Tp + v_off);
-    const int64_t key0 = (int64_t)page * src.T + in_page * kStep;
-    // keys of this step that exist: inside the page, inside the sequence
-    int64_t left = n_keys - key0;
-    const int in_tile = src.T - in_page * kStep;
-    if (left > in_tile) left = in_tile;
-    const int valid = there ? (left > kStep ? kStep : (int)left) : 0;
-    f32x4 sc[R][2];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) sc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
+  for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float mx = -INFINITY, sum = 0.0f;
+  const int per_page = (src.T + kStep - 1) / kStep;
+  const int n_steps = steps_of(src, it.n_keys, kStep, per_page);
+  const int share = it.n_split * 4, mine = it.split * 4 + wk;
+  const int s0 = (int)((int64_t)n_steps * mine / share), s1 = (int)((int64_t)n_steps * (mine + 1) / share);
+  if (s0 < s1) {
+    const int k_off = ((n >> 2) * 8 + (n & 3)) * kHeadDim + g * 8, v_off = n * src.Tp + g * 8;
+    const T* kp = static_cast<const T*>(src.k_pool);
+    const T* vp = static_cast<const T*>(src.v_pool);
+    PageWalk pages;
+    int page = s0 / per_page, in_page = s0 - page * per_page;
+    pages.start(it.list, it.n_list, page);
+    int id = pages.get(page);
+    v8 kf[2][4];
+    auto load_k = [&](int id, int at) {
+      // a page that is not there is read as page 0 and masked
+      const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;
+      const T* p = kp + ((pid * a.heads + it.h) * src.Tp + at * kStep) * (int64_t)kHeadDim + k_off;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < R; ++r) sc[r][t] = Mma<T>::mul(kf[t][st], w.q[r][st], sc[r][t]);
-    // the next step's keys load under this step's softmax and second product
-    if (s + 1 < s1) {
-      if (++in_page == src.spp) {
+        for (int st = 0; st < 4; ++st)
+          kf[t][st] = *reinterpret_cast<const v8*>(p + t * 4 * kHeadDim + st * 32);
+    };
+    load_k(id, in_page);
+    for (int s = s0; s < s1; ++s) {
+      const bool there = id >= 0 && id < src.n_pages;
+      const int64_t pid = there ? id : 0;
+      const T* vb = vp + (pid * a.heads + it.h) * kHeadDim * (int64_t)src.Tp + in_page * kStep;
+      v8 vf[8];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) vf[d] = *reinterpret_cast<const v8*>(vb + d * 16 * (int64_t)src.Tp + v_off);
+      const int64_t key0 = (int64_t)page * src.T + in_page * kStep;
+      // keys of this step that exist: inside the page, inside the sequence
+      int64_t left = it.n_keys - key0;
+      const int in_tile = src.T - in_page * kStep;
+      if (left > in_tile) left = in_tile;
+      const int valid = there ? (left > kStep ? kStep : (int)left) : 0;
+      f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sc[t] = Mma<T>::mul(kf[t][st], q[st], sc[t]);
+      // the next step's keys load under this step's softmax and second product
+      if (s + 1 < s1) {
+        if (++in_page == per_page) {
+          in_page = 0;
+          id = pages.get(++page);
+        }
+        load_k(id, in_page);
+      }
+      const bool partial = OWN && key0 + valid > it.open;  // some row may not see all of them
+      if (valid < kStep || partial) {
+        const int64_t seen = lim - key0;
+        const int most = seen < valid ? (int)(seen < 0 ? 0 : seen) : valid;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (8 * g + i >= most) sc[i >> 2][i & 3] = -INFINITY;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) vf[d] = drop_behind(vf[d], 8 * g, valid);
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i >> 2][i & 3]);
+      top *= a.c;
+      // The maximum only has to keep exp2 in range, so it follows when some row of the wave is 2^8
+      // above it: most steps skip the reductions and the rescaling.
+      if (__any(top > mx + kSlack)) {
+        const float m2 = fmaxf(mx, over_groups_max(top, 16));
+        const float f = m2 == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m2);
+        mx = m2;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] *= f;
+      }
+      const float ms = mx == -INFINITY ? 0.0f : mx;
+      v8 p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(sc[i >> 2][i & 3] * a.c - ms);
+        sum += e;
+        p[i] = (T)e;  // rounded to the pool's type for the matrix product; the sum is of fp32 values
+      }
+      if (partial) {
+        // A key that some rows may not see yet can hold an infinity or a NaN, which 0 * v would
+        // spread to them: such values leave the product and are added to the rows that see them.
+        bool odd = false;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) odd |= drop_odd<T>(vf[d]);
+        if (__any(odd)) {
+#pragma unroll 1
+          for (int key = 0; key < valid; ++key) {
+            const float e = __shfl(pick<T>(p, key & 7), n + 16 * (key >> 3), 64);
+            const bool sees = key0 + key < lim;
+            int tp = src.Tp;
+            asm volatile("" : "+s"(tp));  // keeps 32 addresses out of the registers of the common path
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x = (float)vb[(16 * d + 4 * g + i) * (int64_t)tp + key];
+                if (sees && !__builtin_isfinite(x)) o[d][i] += e * x;
+              }
+              __builtin_amdgcn_sched_barrier(0);  // a rare path: few registers matter more than speed
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[d] = Mma<T>::mul(vf[d], p, o[d]);
+    }
+  }
+  sum = over_groups_sum(sum, 16);
+  // the four waves' shares join in halves through LDS: 32 outputs, m and l of a lane
+#pragma unroll
+  for (int half = 2; half > 0; half >>= 1) {
+    float* at = lds + (wk % half) * 34 * 64 + lane;
+    if (wk >= half && wk < 2 * half) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) at[e * 64] = o[e >> 2][e & 3];
+      at[32 * 64] = mx;
+      at[33 * 64] = sum;
+    }
+    __syncthreads();
+    if (wk < half) {
+      const float m2 = at[32 * 64], l2 = at[33 * 64];
+      const float top = fmaxf(mx, m2), ms = top == -INFINITY ? 0.0f : top;
+      const float x = __builtin_amdgcn_exp2f(mx - ms), y = __builtin_amdgcn_exp2f(m2 - ms);
+      mx = top;
+      sum = sum * x + l2 * y;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e >> 2][e & 3] = o[e >> 2][e & 3] * x + at[e * 64] * y;
+    }
+    __syncthreads();
+  }
+  if (wk > 0 || m >= it.m1) return;
+  T* dst = nullptr;
+  const float inv = row_out<T>(a, it, m, mx, sum, g == 0, &dst);
+#pragma unroll
+  for (int d = 0; d < 8; ++d) put4<T>(a, it, m, 16 * d + 4 * g, o[d], inv, dst);
+}
+
+// ---- more rows: 4 waves of 32 rows share tiles of 64 keys in LDS, on 32x32x16 MFMAs -------------
+// A tile is 16 blocks of K and 16 of V^T, each the A operand of one MFMA in lane order (64 x 16 B), so
+// an operand read is a linear ds_read_b128 and a block is what one direct global -> LDS load writes.
+// Row i of a K block is key 16 (i / 16) + 8 ((i / 4) % 2) + 4 ((i / 8) % 2) + i % 4 of its 32: the 16
+// scores of lane (n, hh) are then row n's keys 8 hh .. 8 hh + 7 and 16 + 8 hh .. 16 + 8 hh + 7.
+constexpr int kBlock = 1024;  // bytes
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <typename T>
+__device__ inline void stage_tile(const T* kt, const T* vt, int Tp, int klane, int vlane, char* dst, int wave) {
+  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kt, (short)0, 0x7fffffff, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vt, (short)0, 0x7fffffff, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int blk = wave * 4 + i, kb = blk >> 3, st = blk & 7;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(dst + blk * kBlock), 16, klane,
+                                             (kb * 32 * kHeadDim + st * 16) * 2, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int blk = wave * 4 + i, db = blk >> 2, kk = blk & 3;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (16 + blk) * kBlock), 16, vlane,
+                                             (db * 32 * Tp + kk * 16) * 2, 0, 0);
+  }
+}
+
+template <typename T, bool OWN>
+__device__ inline void tile_item(const SharedArgs& a, const Source& src, const Item& it, char* lds) {
+  typedef typename Mma<T>::v8 v8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hh = lane >> 5;
+  const int m = it.m0 + 32 * wave + n;
+  const bool busy = it.m0 + 32 * wave < it.m1;  // the wave has rows at all
+  int b, l, gh;
+  row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
+  const int64_t lim = OWN && it.causal ? it.first_lim + l : it.n_keys;
+  v8 q[8];
+  {
+    const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
+                 (int64_t)(it.h * a.group + gh) * a.q_sh + hh * 8;
+#pragma unroll
+    for (int st = 0; st < 8; ++st) q[st] = *reinterpret_cast<const v8*>(p + st * 16);
+  }
+  f32x16 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float mx = -INFINITY, sum = 0.0f;
+  const int per_page = (src.T + kTile - 1) / kTile;
+  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
+  const int t0 = (int)((int64_t)n_tiles * it.split / it.n_split);
+  const int t1 = (int)((int64_t)n_tiles * (it.split + 1) / it.n_split);
+  const int key_row = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+  const int klane = (key_row * kHeadDim + hh * 8) * 2, vlane = (n * src.Tp + hh * 8) * 2;
+  const T* kp = static_cast<const T*>(src.k_pool);
+  const T* vp = static_cast<const T*>(src.v_pool);
+  PageWalk pages;
+  int page = t0 / per_page, in_page = t0 - page * per_page, id = -1;
+  auto tile_k = [&]() {
+    const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;  // a page that is not there: page 0, masked
+    return kp + ((pid * a.heads + it.h) * src.Tp + in_page * kTile) * (int64_t)kHeadDim;
+  };
+  auto tile_v = [&]() {
+    const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;
+    return vp + (pid * a.heads + it.h) * kHeadDim * (int64_t)src.Tp + in_page * kTile;
+  };
+  if (t0 < t1) {
+    pages.start(it.list, it.n_list, page);
+    id = pages.get(page);
+    stage_tile<T>(tile_k(), tile_v(), src.Tp, klane, vlane, lds, wave);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const char* buf = lds + ((t - t0) & 1) * 32 * kBlock;
+    const T* vb = tile_v();
+    const bool there = id >= 0 && id < src.n_pages;
+    const int64_t key0 = (int64_t)page * src.T + in_page * kTile;
+    int64_t left = it.n_keys - key0;
+    const int in_tile = src.T - in_page * kTile;
+    if (left > in_tile) left = in_tile;
+    const int valid = there ? (left > kTile ? kTile : (int)left) : 0;
+    __syncthreads();  // this tile has landed, and nobody reads the other buffer any more
+    if (t + 1 < t1) {
+      if (++in_page == per_page) {
         in_page = 0;
         id = pages.get(++page);
       }
-      load_k(id, in_page);
+      stage_tile<T>(tile_k(), tile_v(), src.Tp, klane, vlane, lds + ((t + 1 - t0) & 1) * 32 * kBlock, wave);
     }
-    const bool partial = key0 + valid > open;  // some row may not see all of them
-    if (valid < kStep || partial) {
+    if (!busy) continue;
+    const v8* kf = reinterpret_cast<const v8*>(buf) + lane;
+    const v8* vf = reinterpret_cast<const v8*>(buf + 16 * kBlock) + lane;
+    f32x16 sc[2];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int64_t seen = lim[r] - key0;
-        const int most = seen < valid ? (int)(seen < 0 ? 0 : seen) : valid;
+    for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (8 * g + 4 * t + i >= most) sc[r][t][i] = -INFINITY;
-      }
-      // what lies behind the last key is not multiplied, whatever the page holds there
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        u32x4 x = __builtin_bit_cast(u32x4, vf[d]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = 8 * g + 2 * e;
-          x[e] = key + 1 < valid ? x[e] : key < valid ? x[e] & 0xffffu : 0u;
-        }
-        vf[d] = __builtin_bit_cast(v8, x);
-      }
+      for (int st = 0; st < 8; ++st) sc[kb] = Mma<T>::mul(kf[(kb * 8 + st) * 64], q[st], sc[kb]);
     }
-    float top[R];
-    bool grow = false;
+    const bool partial = OWN && key0 + valid > it.open, masked = valid < kTile || partial;
+    if (masked) {
+      const int64_t seen = lim - key0;
+      const int most = seen < valid ? (int)(seen < 0 ? 0 : seen) : valid;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float t = sc[r][0][0];
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 1; i < 8; ++i) t = fmaxf(t, sc[r][i >> 2][i & 3]);
-      top[r] = t * c;
-      grow |= top[r] > w.m[r] + kSlack;
+        for (int i = 0; i < 16; ++i)
+          if (32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7) >= most) sc[kb][i] = -INFINITY;
     }
-    // The maximum only has to keep exp2 in range, so it follows when some row of the wave is 2^8
-    // above it: most steps skip the reductions and the rescaling.
-    if (__any(grow)) {
+    float top = sc[0][0];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float m = fmaxf(w.m[r], over_keys_max(top[r]));
-        const float a = m == w.m[r] ? 1.0f : __builtin_amdgcn_exp2f(w.m[r] - m);
-        w.m[r] = m;
-        w.l[r] *= a;
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, sc[i >> 4][i & 15]);
+    top *= a.c;
+    if (__any(top > mx + kSlack)) {  // as in stream_item
+      const float m2 = fmaxf(mx, over_groups_max(top, 32));
+      const float f = m2 == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m2);
+      mx = m2;
+      sum *= f;
 #pragma unroll
-        for (int d = 0; d < 8; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w.o[r][d][i] *= a;
-      }
+      for (int d = 0; d < 4; ++d) o[d] *= f;
     }
-    v8 p[R];
+    const float ms = mx == -INFINITY ? 0.0f : mx;
+    v8 p[4];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float m = w.m[r] == -INFINITY ? 0.0f : w.m[r];
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(sc[r][i >> 2][i & 3] * c - m);
-        sum += e;
-        sc[r][i >> 2][i & 3] = e;
-        p[r][i] = (T)e;  // rounded to the pool's type for the matrix product; l sums it unrounded
-      }
-      w.l[r] += sum;
+    for (int i = 0; i < 32; ++i) {
+      const float e = __builtin_amdgcn_exp2f(sc[i >> 4][i & 15] * a.c - ms);
+      sum += e;
+      p[i >> 3][i & 7] = (T)e;  // rounded to the pool's type; the sum is of fp32 values
     }
-    if (partial) {
-      // A key that some rows may not see yet can hold an infinity or a NaN, which 0 * v would
-      // spread to them: such values leave the product and are added to the rows that see them.
+    if (!masked) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] = Mma<T>::mul(vf[(d * 4 + kk) * 64], p[kk], o[d]);
+    } else {
       bool odd = false;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        u32x4 x = __builtin_bit_cast(u32x4, vf[d]);
+      for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t lo = Mma<T>::kInf, hi = lo << 16;
-          if ((x[e] & lo) == lo) x[e] &= 0xffff0000u, odd = true;
-          if ((x[e] & hi) == hi) x[e] &= 0xffffu, odd = true;
+        for (int d = 0; d < 4; ++d) {
+          v8 x = drop_behind(vf[(d * 4 + kk) * 64], 16 * kk + 8 * hh, valid);
+          if (partial) odd |= drop_odd<T>(x);  // as in stream_item
+          o[d] = Mma<T>::mul(x, p[kk], o[d]);
         }
-        vf[d] = __builtin_bit_cast(v8, x);
-      }
       if (__any(odd)) {
 #pragma unroll 1
         for (int key = 0; key < valid; ++key) {
+          float e = pick<T>(p[0], key & 7);
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            float e = sc[r][0][0];
+          for (int kk = 1; kk < 4; ++kk) e = key >> 4 == kk ? pick<T>(p[kk], key & 7) : e;
+          e = __shfl(e, n + 32 * ((key >> 3) & 1), 64);
+          const bool sees = key0 + key < lim;
+          int tp = src.Tp;
+          asm volatile("" : "+s"(tp));
 #pragma unroll
-            for (int i = 1; i < 8; ++i) e = (key & 7) == i ? sc[r][i >> 2][i & 3] : e;
-            e = __shfl(e, i16 + 16 * (key >> 3), 64);
-            const bool sees = key0 + key < lim[r];
-#pragma unroll
-            for (int d = 0; d < 8; ++d)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x = (float)vb[(16 * d + 4 * g + i) * (int64_t)src.Tp + key];
-                if (sees && !__builtin_isfinite(x)) w.o[r][d][i] += e * x;
-              }
+          for (int i = 0; i < 64; ++i) {
+            const int d = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hh + (i & 3);
+            const float x = (float)vb[d * (int64_t)tp + key];
+            if (sees && !__builtin_isfinite(x)) o[i >> 4][i & 15] += e * x;
+            if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
     }
+  }
+  if (m >= it.m1) return;
+  sum = over_groups_sum(sum, 32);
+  T* dst = nullptr;
+  const float inv = row_out<T>(a, it, m, mx, sum, hh == 0, &dst);
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
+  for (int i = 0; i < 16; ++i) {
+    f32x4 x;
 #pragma unroll
-      for (int r = 0; r < R; ++r) w.o[r][d] = Mma<T>::mul(vf[d], p[r], w.o[r][d]);
+    for (int e = 0; e < 4; ++e) x[e] = o[i >> 2][4 * (i & 3) + e];
+    put4<T>(a, it, m, 32 * (i >> 2) + 8 * (i & 3) + 4 * hh, x, inv, dst);
   }
 }
 
-// One work item: rows [m0, m1) of key head h against a share of a source's steps, by 4 waves: WR of
-// them side by side on 16 R rows each, 4 / WR behind one another along the keys.
-template <typename T, int R, int WR>
-__device__ inline void work_item(const SharedArgs& a, const Source& src, const int32_t* list,
-                                 int n_list, int h, int m0, int m1, int64_t n_keys, int64_t open,
-                                 int64_t first_lim, int n_split, int split, int part, float* lds) {
-  constexpr int WK = 4 / WR;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wr = wave % WR, wk = wave / WR;
-  const int i16 = lane & 15, g = lane >> 4;
-  WaveState<T, R> w;
-  int64_t lim[R];
-  int row_of[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int m = m0 + (wr * R + r) * 16 + i16;
-    row_of[r] = m < m1 ? m : -1;
-    const int mm = m < m1 ? m : m0;
-    const int gh = mm % a.group, bl = mm / a.group, l = bl % a.rows, b = bl / a.rows;
-    // first_lim: own keys that the sequence's row 0 sees, one more for each next row (causal)
-    lim[r] = a.causal && first_lim != INT64_MAX ? first_lim + l : n_keys;
-    const T* q = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
-                 (int64_t)(h * a.group + gh) * a.q_sh + g * 8;
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
-      w.q[r][st] = *reinterpret_cast<const typename Mma<T>::v8*>(q + st * 32);
-#pragma unroll
-    for (int d = 0; d < 8; ++d) w.o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w.m[r] = -INFINITY;
-    w.l[r] = 0.0f;
-  }
-  // steps of the item: whole pages, then what the last page holds
-  const int64_t full = n_keys / src.T;
-  const int rest = (int)(n_keys - full * src.T);
-  const int n_steps = (int)(full * src.spp) + (rest + kStep - 1) / kStep;
-  const int share = n_split * WK, mine = split * WK + wk;
-  const int s0 = (int)((int64_t)n_steps * mine / share), s1 = (int)((int64_t)n_steps * (mine + 1) / share);
-  walk<T, R>(w, src, list, n_list, a.heads, h, n_keys, open, lim, a.c, s0, s1);
-#pragma unroll
-  for (int r = 0; r < R; ++r) w.l[r] = over_keys_sum(w.l[r]);
-  // waves along the keys join in halves through LDS
-  if constexpr (WK > 1) {
-    constexpr int kPer = R * 34 * 64;  // floats of a wave's state: 32 outputs, m and l a lane and tile
-#pragma unroll
-    for (int half = WK / 2; half > 0; half >>= 1) {
-      float* at = lds + ((wk % half) * WR + wr) * kPer + lane;
-      if (wk >= half && wk < 2 * half) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) at[(r * 34 + e) * 64] = w.o[r][e >> 2][e & 3];
-          at[(r * 34 + 32) * 64] = w.m[r];
-          at[(r * 34 + 33) * 64] = w.l[r];
-        }
-      }
-      __syncthreads();
-      if (wk < half) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float m2 = at[(r * 34 + 32) * 64], l2 = at[(r * 34 + 33) * 64];
-          const float m = fmaxf(w.m[r], m2), ms = m == -INFINITY ? 0.0f : m;
-          const float x = __builtin_amdgcn_exp2f(w.m[r] - ms), y = __builtin_amdgcn_exp2f(m2 - ms);
-          w.m[r] = m;
-          w.l[r] = w.l[r] * x + l2 * y;
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            w.o[r][e >> 2][e & 3] = w.o[r][e >> 2][e & 3] * x + at[(r * 34 + e) * 64] * y;
-        }
-      }
-      __syncthreads();
-    }
-    if (wk > 0) return;
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int m = row_of[r];
-    if (m < 0) continue;
-    if (a.direct) {
-      const int gh = m % a.group, bl = m / a.group, l = bl % a.rows, b = bl / a.rows;
-      int fresh = a.rows;
-      if (a.new_lens != nullptr) fresh = a.new_lens[b];
-      const float inv = l < fresh && w.l[r] != 0.0f ? 1.0f / w.l[r] : 0.0f;
-      T* o = static_cast<T*>(a.out) + b * a.o_sb + l * a.o_st + (int64_t)(h * a.group + gh) * a.o_sh + g * 4;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = inv != 0.0f ? (T)(w.o[r][d][i] * inv) : (T)0.0f;
-        *reinterpret_cast<t4*>(o + 16 * d) = x;
-      }
-    } else {
-      const int64_t at = ((int64_t)part * a.heads + h) * a.M + m;
-      float* o = a.part_o + at * kHeadDim + g * 4;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = w.o[r][d];
-      if (g == 0) a.part_ml[at] = float2{w.m[r], w.l[r]};
-    }
-  }
-}
+constexpr int kStreamRows = 16, kTileRows = 128;  // rows of a work item
 
 // The prefix's work items first, dealt so that the row blocks of one (key head, split) run on one
-// XCD and share its L2; then every sequence's own pages.
-template <typename T, int RP, int WRP, int RO, int WRO>
-__global__ __launch_bounds__(256) void attend_shared_kernel(SharedArgs a) {
-  constexpr int kP = WRP < 4 ? 2 * RP * 34 * 64 : 0, kO = WRO < 4 ? 2 * RO * 34 * 64 : 0;
-  __shared__ float lds[(kP > kO ? kP : kO) > 0 ? (kP > kO ? kP : kO) : 1];
+// XCD and share its L2; then every sequence's own pages.  PT, OT: whether the prefix and the own pages
+// go by tiles.
+template <typename T, bool PT, bool OT>
+__global__ __launch_bounds__(256, 2) void attend_shared_kernel(SharedArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[PT || OT ? 64 * kBlock : 2 * 34 * 64 * 4];
   int bid = blockIdx.x;
+  Item it;
   if (bid < a.pre_grid) {
+    constexpr int R = PT ? kTileRows : kStreamRows;
     const int idx = bid >> 3, pair = (idx / a.pre_rb) * 8 + (bid & 7), rb = idx % a.pre_rb;
     if (pair >= a.heads * a.pre_splits) return;
-    const int h = pair % a.heads, split = pair / a.heads;
-    const int m0 = rb * 16 * RP * WRP;
-    const int m1 = m0 + 16 * RP * WRP < a.M ? m0 + 16 * RP * WRP : a.M;
-    const int64_t n_list = (a.pre_tokens + a.pre.T - 1) / a.pre.T;
-    work_item<T, RP, WRP>(a, a.pre, a.pre_pages, (int)n_list, h, m0, m1, a.pre_tokens, a.pre_tokens,
-                          INT64_MAX, a.pre_splits, split, split, lds);
+    it.h = pair % a.heads;
+    it.split = it.part = pair / a.heads;
+    it.n_split = a.pre_splits;
+    it.m0 = rb * R;
+    it.m1 = it.m0 + R < a.M ? it.m0 + R : a.M;
+    it.list = a.pre_pages;
+    it.n_list = (int)((a.pre_tokens + a.pre.T - 1) / a.pre.T);
+    it.n_keys = it.open = a.pre_tokens;
+    it.first_lim = 0;
+    it.causal = false;
+    if constexpr (PT) tile_item<T, false>(a, a.pre, it, lds);
+    else stream_item<T, false>(a, a.pre, it, reinterpret_cast<float*>(lds));
     return;
   }
+  constexpr int R = OT ? kTileRows : kStreamRows;
   bid -= a.pre_grid;
-  const int split = bid % a.own_splits;
+  it.split = bid % a.own_splits;
   bid /= a.own_splits;
   const int rb = bid % a.own_rb;
   bid /= a.own_rb;
-  const int h = bid % a.heads, b = bid / a.heads;
-  const int per = a.rows * a.group;
-  const int m0 = b * per + rb * 16 * RO * WRO;
-  const int m1 = m0 + 16 * RO * WRO < (b + 1) * per ? m0 + 16 * RO * WRO : (b + 1) * per;
-  int fresh = a.rows;
-  if (a.new_lens != nullptr) {
-    fresh = a.new_lens[b];
-    fresh = fresh < 0 ? 0 : fresh > a.rows ? a.rows : fresh;
-  }
-  int64_t n_keys = a.lengths[b];
-  const int64_t cap = (int64_t)a.width * a.own.T;
-  // rows of a causal sequence: row l sees lengths - fresh + l + 1 keys, whatever the table holds
-  int64_t first_lim = n_keys - fresh + 1;
-  n_keys = n_keys < 0 ? 0 : n_keys > cap ? cap : n_keys;
-  const int64_t open = a.causal ? first_lim + (m0 - b * per) / a.group : n_keys;
-  work_item<T, RO, WRO>(a, a.own, a.tables + b * a.table_st, a.width, h, m0, m1, n_keys, open, first_lim,
-                        a.own_splits, split, a.pre_splits + split, lds);
+  it.h = bid % a.heads;
+  const int b = bid / a.heads, per = a.rows * a.group;
+  it.n_split = a.own_splits;
+  it.part = a.pre_splits + it.split;
+  it.m0 = b * per + rb * R;
+  it.m1 = it.m0 + R < (b + 1) * per ? it.m0 + R : (b + 1) * per;
+  it.list = a.tables + b * a.table_st;
+  it.n_list = a.width;
+  it.causal = a.causal;
+  // row l of a causal sequence sees lengths - fresh + l + 1 keys; keys past the table do not exist
+  const int fresh = fresh_rows(a, b), l0 = rb * R / a.group, l1 = (it.m1 - 1 - b * per) / a.group;
+  const int64_t length = a.lengths[b], cap = (int64_t)a.width * a.own.T;
+  it.first_lim = length - fresh + 1;
+  it.n_keys = a.causal && it.first_lim + l1 < length ? it.first_lim + l1 : length;
+  if (it.n_keys > cap) it.n_keys = cap;
+  if (it.n_keys < 0 || l0 >= fresh) it.n_keys = 0;  // no row of the item is a new token
+  it.open = a.causal ? it.first_lim + l0 : it.n_keys;
+  if constexpr (OT) tile_item<T, true>(a, a.own, it, lds);
+  else stream_item<T, true>(a, a.own, it, reinterpret_cast<float*>(lds));
 }
 
 // One wave per (row, key head): the parts' weights, then their outputs, a lane two channels.
@@ -692,7 +874,7 @@ int common_errors(const char* fn, int dtype, int head_dim, int batch, int rows, 
               q_heads, kv_heads);
     return SKV_E_ARG;
   }
-  if (n_pages <= 0 || page_tokens <= 0 || page_tokens > (1 << 24)) {
+  if (n_pages <= 0 || page_tokens <= 0 || page_tokens > (1 << 20)) {
     set_error("%s: bad pool (%d pages of %d tokens)", fn, n_pages, page_tokens);
     return SKV_E_ARG;
   }
@@ -704,17 +886,12 @@ int common_errors(const char* fn, int dtype, int head_dim, int batch, int rows, 
   return SKV_OK;
 }
 
-// The launch of an attention: row tiles and waves of both kinds of work item, and the splits.
+// The launch of an attention: whether each kind of work item goes by tiles, and the splits.
 struct SharedPlan {
-  int pre_kind, own_kind;  // 0: 16 rows, waves along the keys; 1: 64 rows; 2: 128 rows
+  bool pre_tiles, own_tiles;
   int pre_rb, pre_splits, pre_grid, own_rb, own_splits, own_grid, parts;
   int64_t bytes;
 };
-
-constexpr int kKindRows[3] = {16, 64, 128};
-constexpr int kKindWK[3] = {4, 2, 1};  // waves along the keys
-
-int kind_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 64 ? 1 : 2; }
 
 int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) {
   const int group = d->q_heads / d->kv_heads;
@@ -725,30 +902,27 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
   }
   *p = SharedPlan{};
   const bool pre = d->prefix_tokens > 0, own = d->table_width > 0;
-  p->pre_kind = kind_of(M);
-  p->own_kind = kind_of(per);
-  if (!pre) p->pre_kind = p->own_kind;
+  p->own_tiles = per > kStreamRows;
+  p->pre_tiles = pre ? M > kStreamRows : p->own_tiles;
+  const int pre_rows = p->pre_tiles ? kTileRows : kStreamRows, own_rows = p->own_tiles ? kTileRows : kStreamRows;
   const int64_t cu = cu_count();
-  // steps of 32 keys that one wave would take, over all work items
-  const int64_t pre_steps = pre ? (d->prefix_tokens / d->prefix_page_tokens) *
-                                          ((d->prefix_page_tokens + kStep - 1) / kStep) +
-                                      (d->prefix_tokens % d->prefix_page_tokens + kStep - 1) / kStep
-                                : 0;
-  const int64_t own_steps = own ? (int64_t)d->table_width * ((d->page_tokens + kStep - 1) / kStep) : 0;
-  p->pre_rb = pre ? (int)((M + kKindRows[p->pre_kind] - 1) / kKindRows[p->pre_kind]) : 0;
-  p->own_rb = own ? (int)((per + kKindRows[p->own_kind] - 1) / kKindRows[p->own_kind]) : 0;
+  auto tiles = [](int64_t tokens, int64_t page) {
+    return tokens / page * ((page + kTile - 1) / kTile) + (tokens % page + kTile - 1) / kTile;
+  };
+  const int64_t pre_tiles = pre ? tiles(d->prefix_tokens, d->prefix_page_tokens) : 0;
+  const int64_t own_tiles = own ? tiles((int64_t)d->table_width * d->page_tokens, d->page_tokens) : 0;
+  p->pre_rb = pre ? (int)((M + pre_rows - 1) / pre_rows) : 0;
+  p->own_rb = own ? (int)((per + own_rows - 1) / own_rows) : 0;
   const int64_t pre_items = (int64_t)p->pre_rb * d->kv_heads;
   const int64_t own_items = (int64_t)p->own_rb * d->kv_heads * d->batch;
-  const int64_t wave_steps = pre_items * ((pre_steps + kKindWK[p->pre_kind] - 1) / kKindWK[p->pre_kind]) +
-                             own_items * ((own_steps + kKindWK[p->own_kind] - 1) / kKindWK[p->own_kind]);
-  int64_t share = (wave_steps + 2 * cu - 1) / (2 * cu);  // steps of a wave with two workgroups a CU
-  if (share < 4) share = 4;
-  auto splits = [&](int64_t steps, int kind) -> int {
-    const int64_t s = (steps + share * kKindWK[kind] - 1) / (share * kKindWK[kind]);
+  int64_t share = (pre_items * pre_tiles + own_items * own_tiles + 2 * cu - 1) / (2 * cu);
+  if (share < 8) share = 8;
+  auto splits = [&](int64_t n) -> int {
+    const int64_t s = (n + share - 1) / share;
     return (int)(s < 1 ? 1 : s > 1024 ? 1024 : s);
   };
-  p->pre_splits = pre ? splits(pre_steps, p->pre_kind) : 0;
-  p->own_splits = own ? splits(own_steps, p->own_kind) : 0;
+  p->pre_splits = pre ? splits(pre_tiles) : 0;
+  p->own_splits = own ? splits(own_tiles) : 0;
   p->parts = p->pre_splits + p->own_splits;
   const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits;
   const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, own_grid = own_items * p->own_splits;
@@ -784,7 +958,7 @@ int check_shared(const char* fn, const skv_attend_shared_desc* d) {
   if (d->prefix_tokens < 0 ||
       (d->prefix_tokens > 0 &&
        (!pool_ok(d->prefix_k_pool, d->prefix_v_pool) || !d->prefix_pages || d->prefix_n_pages <= 0 ||
-        d->prefix_page_tokens <= 0 || d->prefix_page_tokens > (1 << 24) ||
+        d->prefix_page_tokens <= 0 || d->prefix_page_tokens > (1 << 20) ||
         d->prefix_tokens >= ((int64_t)1 << 31)))) {
     set_error("%s: bad prefix (%lld tokens in pages of %d)", fn, (long long)d->prefix_tokens,
               d->prefix_page_tokens);
@@ -800,18 +974,9 @@ int check_shared(const char* fn, const skv_attend_shared_desc* d) {
 template <typename T>
 void launch_shared(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.pre_grid + p.own_grid)), block(256);
-#define SKV_KINDS(P, O, RP, WRP, RO, WRO)                                                        \
-  if (p.pre_kind == P && p.own_kind == O) {                                                      \
-    hipLaunchKernelGGL((attend_shared_kernel<T, RP, WRP, RO, WRO>), grid, block, 0, s, a);       \
-    return;                                                                                      \
-  }
-  SKV_KINDS(0, 0, 1, 1, 1, 1)
-  SKV_KINDS(1, 0, 2, 2, 1, 1)
-  SKV_KINDS(1, 1, 2, 2, 2, 2)
-  SKV_KINDS(2, 0, 2, 4, 1, 1)
-  SKV_KINDS(2, 1, 2, 4, 2, 2)
-  SKV_KINDS(2, 2, 2, 4, 2, 4)
-#undef SKV_KINDS
+  if (!p.pre_tiles) hipLaunchKernelGGL((attend_shared_kernel<T, false, false>), grid, block, 0, s, a);
+  else if (!p.own_tiles) hipLaunchKernelGGL((attend_shared_kernel<T, true, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((attend_shared_kernel<T, true, true>), grid, block, 0, s, a);
 }
 
 }  // namespace
@@ -943,11 +1108,10 @@ extern "C" int skv_attend_shared(const skv_attend_shared_desc* d, skv_stream_t s
   SharedArgs a{};
   a.q = d->q, a.q_sb = d->q_sb, a.q_st = d->q_st, a.q_sh = d->q_sh;
   a.out = d->out, a.o_sb = d->out_sb, a.o_st = d->out_st, a.o_sh = d->out_sh;
-  a.own = Source{d->k_pool, d->v_pool, d->n_pages, d->page_tokens, padded_tokens(d->page_tokens),
-                 (d->page_tokens + kStep - 1) / kStep};
+  a.own = Source{d->k_pool, d->v_pool, d->n_pages, d->page_tokens, padded_tokens(d->page_tokens)};
   if (d->prefix_tokens > 0)
     a.pre = Source{d->prefix_k_pool, d->prefix_v_pool, d->prefix_n_pages, d->prefix_page_tokens,
-                   padded_tokens(d->prefix_page_tokens), (d->prefix_page_tokens + kStep - 1) / kStep};
+                   padded_tokens(d->prefix_page_tokens)};
   a.pre_pages = d->prefix_pages, a.pre_tokens = d->prefix_tokens;
   a.tables = d->tables, a.table_st = d->table_stride, a.width = d->table_width;
   a.lengths = d->lengths, a.new_lens = d->new_lens;
