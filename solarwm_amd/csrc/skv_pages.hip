@@ -224,6 +224,10 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
 // V straight from memory to registers, bound by bytes.  More rows share: 4 waves of 32 rows read
 // tiles of 64 keys that the workgroup stages in LDS, bound by the matrix cores.
 // ---------------------------------------------------------------------------------------------
+constexpr int kWaves = 8;    // of a workgroup: one workgroup a CU, two waves a SIMD
+// rows of a work item that streams (0) or goes by 1 or 2 tiles a round, and how many rows go
+constexpr int kind_rows(int kind) { return kind == 0 ? 16 : 32 * kWaves / kind; }
+constexpr int kind_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 128 ? 2 : 1; }
 constexpr int kStep = 32;    // keys of a streaming step
 constexpr float kSlack = 8;  // the running maximum may lag the true one by 2^8 (see below)
 
@@ -249,7 +253,7 @@ struct SharedArgs {
   float c;       // softmax_scale * log2(e)
   int M;         // batch * rows * group
   int pre_rb, pre_splits, pre_grid;  // row blocks, key splits and workgroups of the prefix
-  int own_rb, own_splits;            // row blocks of a sequence, key splits
+  int own_rb, own_splits, own_items, own_waves;  // row blocks of a sequence, key splits; waves of an item
   int direct;    // one part only: workgroups write out themselves
   float* part_o;   // [part][heads][M][128]
   float2* part_ml; // [part][heads][M]
@@ -325,14 +329,21 @@ __device__ inline bool drop_odd(typename Mma<T>::v8& v) {
   return odd;
 }
 
-// Element i of a piece, i known at run time only.
+// Ones where a piece holds +infinity (kind 0), -infinity (1) or NaN (2), zeros elsewhere.
 template <typename T>
-__device__ inline float pick(typename Mma<T>::v8 v, int i) {
-  const u32x4 x = __builtin_bit_cast(u32x4, v);
-  const uint32_t w = i < 4 ? (i < 2 ? x[0] : x[1]) : (i < 6 ? x[2] : x[3]);
-  const uint16_t bits = (uint16_t)(i & 1 ? w >> 16 : w);
-  return (float)__builtin_bit_cast(T, bits);
+__device__ inline typename Mma<T>::v8 marks(typename Mma<T>::v8 v, int kind) {
+  u32x4 x = __builtin_bit_cast(u32x4, v);
+  const uint32_t one = __builtin_bit_cast(uint16_t, (T)1.0f), want = Mma<T>::kInf | (kind == 1 ? 0x8000u : 0u);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = x[e] & 0xffffu, hi = x[e] >> 16;
+    const bool l = kind == 2 ? (lo & 0x7fffu) > Mma<T>::kInf : lo == want;
+    const bool h = kind == 2 ? (hi & 0x7fffu) > Mma<T>::kInf : hi == want;
+    x[e] = (l ? one : 0u) | (h ? one << 16 : 0u);
+  }
+  return __builtin_bit_cast(typename Mma<T>::v8, x);
 }
+__device__ inline float marked(int kind) { return kind == 2 ? __builtin_nanf("") : kind == 1 ? -INFINITY : INFINITY; }
 
 // A work item's page list, 64 entries in a vector register at a time.
 struct PageWalk {
@@ -347,6 +358,8 @@ struct PageWalk {
     base = page;
     const int i = page + (int)(threadIdx.x & 63);
     ids = i < n ? list[i] : -1;
+    // waited for here, not wherever the paths meet again: there it would drain the tiles under way
+    asm volatile("" : "+v"(ids));
   }
   __device__ int get(int page) {
     if (page - base >= 64) fill(page);
@@ -406,15 +419,17 @@ __device__ inline float row_out(const SharedArgs& a, const Item& it, int m, floa
 // ---- at most 16 rows: a wave streams its own keys, 32 a step, on 16x16x32 MFMAs ----------------
 // Row i of S tile t is key (i / 4) * 8 + 4 t + i % 4 of the step; lane (n, g) holds row n's keys
 // 8 g .. 8 g + 7.
+// `waves` of the workgroup (1, 2, 4 or 8, the same for all its items) work on one item, this one of them
+// being number wk.  All waves of the workgroup come here: those without an item with m0 == m1.
 template <typename T, bool OWN>
-__device__ inline void stream_item(const SharedArgs& a, const Source& src, const Item& it, float* lds) {
+__device__ inline void stream_item(const SharedArgs& a, const Source& src, const Item& it, int waves, float* lds) {
   typedef typename Mma<T>::v8 v8;
-  const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = wave & (waves - 1), n = lane & 15, g = lane >> 4;
   const int m = it.m0 + n;
   int b, l, gh;
   row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
-  const int64_t lim = OWN && it.causal ? it.first_lim + l : it.n_keys;
+  const int lim = (int)(OWN && it.causal ? it.first_lim + l : it.n_keys);
   v8 q[4];
   {
     const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
@@ -428,7 +443,7 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
   float mx = -INFINITY, sum = 0.0f;
   const int per_page = (src.T + kStep - 1) / kStep;
   const int n_steps = steps_of(src, it.n_keys, kStep, per_page);
-  const int share = it.n_split * 4, mine = it.split * 4 + wk;
+  const int share = it.n_split * waves, mine = it.split * waves + wk;
   const int s0 = (int)((int64_t)n_steps * mine / share), s1 = (int)((int64_t)n_steps * (mine + 1) / share);
   if (s0 < s1) {
     const int k_off = ((n >> 2) * 8 + (n & 3)) * kHeadDim + g * 8, v_off = n * src.Tp + g * 8;
@@ -478,8 +493,7 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
       }
       const bool partial = OWN && key0 + valid > it.open;  // some row may not see all of them
       if (valid < kStep || partial) {
-        const int64_t seen = lim - key0;
-        const int most = seen < valid ? (int)(seen < 0 ? 0 : seen) : valid;
+        const int seen = lim - (int)key0, most = seen < valid ? seen : valid;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (8 * g + i >= most) sc[i >> 2][i & 3] = -INFINITY;
@@ -509,39 +523,38 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
         p[i] = (T)e;  // rounded to the pool's type for the matrix product; the sum is of fp32 values
       }
       if (partial) {
-        // A key that some rows may not see yet can hold an infinity or a NaN, which 0 * v would
-        // spread to them: such values leave the product and are added to the rows that see them.
+        // A key that some rows may not see yet can hold an infinity or a NaN, which 0 * v would spread
+        // to them: such values leave the product, and the rows that see one (their probability times a
+        // mark is not zero) get it.
+        v8 clean[8];
         bool odd = false;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) odd |= drop_odd<T>(vf[d]);
+        for (int d = 0; d < 8; ++d) {
+          clean[d] = vf[d];
+          odd |= drop_odd<T>(clean[d]);
+        }
         if (__any(odd)) {
 #pragma unroll 1
-          for (int key = 0; key < valid; ++key) {
-            const float e = __shfl(pick<T>(p, key & 7), n + 16 * (key >> 3), 64);
-            const bool sees = key0 + key < lim;
-            int tp = src.Tp;
-            asm volatile("" : "+s"(tp));  // keeps 32 addresses out of the registers of the common path
+          for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
+              const f32x4 seen = Mma<T>::mul(marks<T>(vf[d], kind), p, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x = (float)vb[(16 * d + 4 * g + i) * (int64_t)tp + key];
-                if (sees && !__builtin_isfinite(x)) o[d][i] += e * x;
-              }
-              __builtin_amdgcn_sched_barrier(0);  // a rare path: few registers matter more than speed
+              for (int i = 0; i < 4; ++i)
+                if (seen[i] > 0.0f) o[d][i] += marked(kind);
             }
-          }
         }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) vf[d] = clean[d];
       }
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[d] = Mma<T>::mul(vf[d], p, o[d]);
     }
   }
   sum = over_groups_sum(sum, 16);
-  // the four waves' shares join in halves through LDS: 32 outputs, m and l of a lane
-#pragma unroll
-  for (int half = 2; half > 0; half >>= 1) {
-    float* at = lds + (wk % half) * 34 * 64 + lane;
+  // the waves' shares join in halves through LDS: 32 outputs, m and l of a lane
+  for (int half = waves >> 1; half > 0; half >>= 1) {
+    float* at = lds + (wave / waves * (waves >> 1) + (wk & (half - 1))) * 34 * 64 + lane;
     if (wk >= half && wk < 2 * half) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) at[e * 64] = o[e >> 2][e & 3];
@@ -567,198 +580,332 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
   for (int d = 0; d < 8; ++d) put4<T>(a, it, m, 16 * d + 4 * g, o[d], inv, dst);
 }
 
-// ---- more rows: 4 waves of 32 rows share tiles of 64 keys in LDS, on 32x32x16 MFMAs -------------
-// A tile is 16 blocks of K and 16 of V^T, each the A operand of one MFMA in lane order (64 x 16 B), so
-// an operand read is a linear ds_read_b128 and a block is what one direct global -> LDS load writes.
-// Row i of a K block is key 16 (i / 16) + 8 ((i / 4) % 2) + 4 ((i / 8) % 2) + i % 4 of its 32: the 16
-// scores of lane (n, hh) are then row n's keys 8 hh .. 8 hh + 7 and 16 + 8 hh .. 16 + 8 hh + 7.
-constexpr int kBlock = 1024;  // bytes
+// ---- more rows: waves of 32 rows share tiles of 64 keys in LDS, on 32x32x16 MFMAs ---------------
+// K lies in LDS as two halves of 64 channels, 128 B a key, V^T as 128 B (64 keys) a channel; a direct
+// global -> LDS load fills 8 such rows, so it reads whole 128 B lines.  16 B piece c of row r holds piece
+// c ^ (r / 2) % 8 of the row in memory: the 16 lanes that an operand read serves at once then fall on
+// different banks.  Row i of a K operand is key 16 (i / 16) + 8 ((i / 4) % 2) + 4 ((i / 8) % 2) + i % 4
+// of its 32: the 16 scores of lane (n, hh) are then row n's keys 8 hh .. 8 hh + 7 and 16 + 8 hh .. + 7.
+//
+// Two waves a SIMD: one's softmax runs under the other's products.
+constexpr int kBlock = 1024;  // bytes that a wave's direct load fills
+constexpr int kRing = 4;       // tiles in LDS: one in use, three on their way
+constexpr int kTileLds = kRing * 32 * kBlock;
 typedef __attribute__((address_space(3))) void lds_void;
 
+// Where a tile lies and what of it exists.
+struct TileAt {
+  int64_t base;  // (page * heads + head), page 0 for one that is not there
+  int64_t key0;  // number of its first key
+  int tok0;      // its first token in the page
+  int valid;     // keys that exist
+};
+
+struct TileWalk {
+  PageWalk pages;
+  int page, in_page, per_page, id;
+  __device__ void start(const Item& it, int per, int tile) {
+    per_page = per;
+    page = tile / per;
+    in_page = tile - page * per;
+    pages.start(it.list, it.n_list, page);
+    id = pages.get(page);
+  }
+  __device__ void next() {
+    if (++in_page == per_page) {
+      in_page = 0;
+      id = pages.get(++page);
+    }
+  }
+  __device__ TileAt at(const Source& src, const Item& it, int heads) const {
+    TileAt x;
+    const bool there = id >= 0 && id < src.n_pages;
+    x.base = (int64_t)(there ? id : 0) * heads + it.h;
+    x.tok0 = in_page * kTile;
+    x.key0 = (int64_t)page * src.T + x.tok0;
+    int64_t left = it.n_keys - x.key0;
+    if (left > src.T - x.tok0) left = src.T - x.tok0;
+    x.valid = there ? (left > kTile ? kTile : (int)left) : 0;
+    return x;
+  }
+};
+
+// A wave's share of a tile: 8 keys of K and twice 8 channels of V^T.  `lane` and `dst` are its own.
 template <typename T>
-__device__ inline void stage_tile(const T* kt, const T* vt, int Tp, int klane, int vlane, char* dst, int wave) {
+__device__ inline void stage_tile(const Source& src, const TileAt& x, int klane, int vlane, char* dst, int wave) {
+  const T* kt = static_cast<const T*>(src.k_pool) + (x.base * src.Tp + x.tok0) * kHeadDim;
+  const T* vt = static_cast<const T*>(src.v_pool) + x.base * kHeadDim * (int64_t)src.Tp + x.tok0;
   const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kt, (short)0, 0x7fffffff, 0x00020000);
   const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vt, (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int blk = wave * 4 + i, kb = blk >> 3, st = blk & 7;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(dst + blk * kBlock), 16, klane,
-                                             (kb * 32 * kHeadDim + st * 16) * 2, 0, 0);
-  }
+  for (int i = 0; i < 2; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(dst + (8 * i + wave) * kBlock), 16, klane,
+                                             (8 * wave * kHeadDim + 64 * i) * 2, 0, 0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int blk = wave * 4 + i, db = blk >> 2, kk = blk & 3;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (16 + blk) * kBlock), 16, vlane,
-                                             (db * 32 * Tp + kk * 16) * 2, 0, 0);
+  for (int i = 0; i < 2; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (16 + 8 * i + wave) * kBlock), 16, vlane,
+                                             8 * (wave + 8 * i) * src.Tp * 2, 0, 0);
+}
+
+// 16 products with their LDS operands read four ahead.
+__device__ inline void ahead_of_products() {
+  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+  for (int i = 0; i < 12; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+}
+
+template <typename T>
+struct TileState {
+  typename Mma<T>::v8 q[8];
+  f32x16 o[4];
+  float mx, sum;
+};
+
+// The probabilities of a tile at the running maximum, without looking for the tile's own: only when a
+// lane's sum leaves [0, 2^8] (or the row has no maximum yet) does the wave take the true maximum,
+// rescale what it has and form the tile's probabilities again.
+template <typename T>
+__device__ inline float probs(const f32x16 (&sc)[2], float c, float mx, typename Mma<T>::v8 (&p)[4]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float e = __builtin_amdgcn_exp2f(sc[i >> 4][i & 15] * c - mx);
+    sum += e;
+    p[i >> 3][i & 7] = (T)e;  // rounded to the pool's type; the sum is of fp32 values
+  }
+  return sum;
+}
+
+template <typename T>
+__device__ inline void settle(TileState<T>& w, const f32x16 (&sc)[2], float c, float sum, typename Mma<T>::v8 (&p)[4]) {
+  if (__any(!(sum <= 256.0f) || w.mx == -INFINITY)) {
+    float top = sc[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, sc[i >> 4][i & 15]);
+    top = over_groups_max(top, 32) * c;
+    const float m2 = fmaxf(w.mx, top);
+    const float f = m2 == w.mx ? 1.0f : __builtin_amdgcn_exp2f(w.mx - m2);
+    w.mx = m2;
+    w.sum *= f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) w.o[d] *= f;
+    sum = probs<T>(sc, c, m2 == -INFINITY ? 0.0f : m2, p);
+  }
+  w.sum += sum;
+}
+
+// The second product of a tile that has keys which do not exist, or (OWN) that some rows do not see.
+template <typename T, bool OWN>
+__device__ inline void masked_pv(TileState<T>& w, const TileAt& x, bool partial, const char* vt,
+                                 const int (&piece)[4], const typename Mma<T>::v8 (&p)[4]) {
+  typedef typename Mma<T>::v8 v8;
+  const int hh = (threadIdx.x & 63) >> 5;
+  bool odd = false;
+  v8 v[4], ahead[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) v[d] = *reinterpret_cast<const v8*>(vt + piece[0] + d * 4 * kBlock);
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    if (16 * kk >= x.valid) break;
+    if (kk < 3 && 16 * kk + 16 < x.valid) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) ahead[d] = *reinterpret_cast<const v8*>(vt + piece[kk + 1] + d * 4 * kBlock);
+    }
+    if (16 * kk + 16 > x.valid) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = drop_behind(v[d], 16 * kk + 8 * hh, x.valid);
+    }
+    if (partial) {  // as in stream_item
+#pragma unroll
+      for (int d = 0; d < 4; ++d) odd |= drop_odd<T>(v[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) w.o[d] = Mma<T>::mul(v[d], p[kk], w.o[d]);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) v[d] = ahead[d];
+  }
+  // The products' results are copied on some of the paths from here, which hipcc has left short of their
+  // wait states: they wait here.
+  asm volatile("s_nop 11" : "+v"(w.o[0]), "+v"(w.o[1]), "+v"(w.o[2]), "+v"(w.o[3]));
+  if (OWN && __any(odd)) {
+#pragma unroll 1
+    for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        f32x16 seen;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) seen[i] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const v8 raw = *reinterpret_cast<const v8*>(vt + piece[kk] + d * 4 * kBlock);
+          seen = Mma<T>::mul(marks<T>(drop_behind(raw, 16 * kk + 8 * hh, x.valid), kind), p[kk], seen);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (seen[i] > 0.0f) w.o[d][i] += marked(kind);
+      }
   }
 }
 
-template <typename T, bool OWN>
+// WK tiles a round: with 2, waves 0..3 work on the first and waves 4..7 on the second, on the same 128
+// rows; with 1, all eight on one tile and 256 rows.
+template <typename T, int WK, bool OWN>
 __device__ inline void tile_item(const SharedArgs& a, const Source& src, const Item& it, char* lds) {
   typedef typename Mma<T>::v8 v8;
+  constexpr int kRows = kWaves / WK;  // waves side by side
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 31, hh = lane >> 5;
-  const int m = it.m0 + 32 * wave + n;
-  const bool busy = it.m0 + 32 * wave < it.m1;  // the wave has rows at all
+  const int n = lane & 31, hh = lane >> 5, wr = wave % kRows, wk = wave / kRows;
+  const int m = it.m0 + 32 * wr + n;
+  const bool busy = it.m0 + 32 * wr < it.m1;  // the wave has rows at all
   int b, l, gh;
   row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
-  const int64_t lim = OWN && it.causal ? it.first_lim + l : it.n_keys;
-  v8 q[8];
+  const int lim = (int)(OWN && it.causal ? it.first_lim + l : it.n_keys);
+  TileState<T> w;
   {
     const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
                  (int64_t)(it.h * a.group + gh) * a.q_sh + hh * 8;
 #pragma unroll
-    for (int st = 0; st < 8; ++st) q[st] = *reinterpret_cast<const v8*>(p + st * 16);
+    for (int st = 0; st < 8; ++st) w.q[st] = *reinterpret_cast<const v8*>(p + st * 16);
+    // the queries' own wait, ahead of the loop's counted ones
+#pragma unroll
+    for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
   }
-  f32x16 o[4];
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-  float mx = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
+  w.mx = -INFINITY;
+  w.sum = 0.0f;
   const int per_page = (src.T + kTile - 1) / kTile;
   const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
   const int t0 = (int)((int64_t)n_tiles * it.split / it.n_split);
-  const int t1 = (int)((int64_t)n_tiles * (it.split + 1) / it.n_split);
+  const int n_own = (int)((int64_t)n_tiles * (it.split + 1) / it.n_split) - t0;
   const int key_row = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
-  const int klane = (key_row * kHeadDim + hh * 8) * 2, vlane = (n * src.Tp + hh * 8) * 2;
-  const T* kp = static_cast<const T*>(src.k_pool);
-  const T* vp = static_cast<const T*>(src.v_pool);
-  PageWalk pages;
-  int page = t0 / per_page, in_page = t0 - page * per_page, id = -1;
-  auto tile_k = [&]() {
-    const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;  // a page that is not there: page 0, masked
-    return kp + ((pid * a.heads + it.h) * src.Tp + in_page * kTile) * (int64_t)kHeadDim;
-  };
-  auto tile_v = [&]() {
-    const int64_t pid = id < 0 || id >= src.n_pages ? 0 : id;
-    return vp + (pid * a.heads + it.h) * kHeadDim * (int64_t)src.Tp + in_page * kTile;
-  };
-  if (t0 < t1) {
-    pages.start(it.list, it.n_list, page);
-    id = pages.get(page);
-    stage_tile<T>(tile_k(), tile_v(), src.Tp, klane, vlane, lds, wave);
+  // loads: lane (r, c) of a wave takes row r of its 8, piece c ^ (row / 2) % 8
+  const int from = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
+  const int klane = ((lane >> 3) * kHeadDim + from * 8) * 2, vlane = ((lane >> 3) * src.Tp + from * 8) * 2;
+  // operand reads: where pieces 2 i + hh of the lane's K row and V^T row lie
+  int kpiece[4], vpiece[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    kpiece[i] = key_row * 128 + (((2 * i + hh) ^ ((key_row >> 1) & 7)) * 16);
+    vpiece[i] = n * 128 + (((2 * i + hh) ^ ((n >> 1) & 7)) * 16);
   }
-  for (int t = t0; t < t1; ++t) {
-    const char* buf = lds + ((t - t0) & 1) * 32 * kBlock;
-    const T* vb = tile_v();
-    const bool there = id >= 0 && id < src.n_pages;
-    const int64_t key0 = (int64_t)page * src.T + in_page * kTile;
-    int64_t left = it.n_keys - key0;
-    const int in_tile = src.T - in_page * kTile;
-    if (left > in_tile) left = in_tile;
-    const int valid = there ? (left > kTile ? kTile : (int)left) : 0;
-    __syncthreads();  // this tile has landed, and nobody reads the other buffer any more
-    if (t + 1 < t1) {
-      if (++in_page == per_page) {
-        in_page = 0;
-        id = pages.get(++page);
+  TileWalk walk;  // at the tile that loads last
+  TileAt ring[kRing - WK];  // the tiles in use and those on their way
+  auto stage = [&](TileAt& x, int t) {
+    if (t == 0) walk.start(it, per_page, t0);
+    else walk.next();
+    x = walk.at(src, it, a.heads);
+    char* const to = lds + (t & (kRing - 1)) * 32 * kBlock;
+    stage_tile<T>(src, x, klane, vlane, to, wave);
+  };
+#pragma unroll
+  for (int i = 0; i < kRing - WK; ++i) {
+    ring[i] = TileAt{};
+    if (i < n_own) stage(ring[i], i);
+  }
+  for (int t = 0; t < n_own; t += WK) {
+    // This round's tiles have landed (a wave's loads land in order: what was issued after them may
+    // still be under way), and everybody is done with the round before, whose buffers load next.
+    constexpr int kLoads = 4;  // of a wave and tile
+    if (WK == 1 && t + 2 < n_own) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+    else if (WK == 1 && t + 1 < n_own) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const TileAt cur = WK == 2 && wk == 1 ? ring[1] : ring[0];
+#pragma unroll
+    for (int i = 0; i + WK < kRing - WK; ++i) ring[i] = ring[i + WK];
+#pragma unroll
+    for (int i = 0; i < WK; ++i)
+      if (t + kRing - WK + i < n_own) stage(ring[kRing - 2 * WK + i], t + kRing - WK + i);
+    const char* const kt = lds + ((t + wk) & (kRing - 1)) * 32 * kBlock;
+    const char* const vt = kt + 16 * kBlock;
+    if (busy && t + wk < n_own) {
+      f32x16 sc[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sc[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(kt + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
+                                w.q[i >> 1], sc[i & 1]);
+      ahead_of_products();
+      const bool partial = OWN && cur.key0 + cur.valid > it.open, masked = cur.valid < kTile || partial;
+      if (masked) {
+        const int seen = lim - (int)cur.key0;
+        int most = (seen < cur.valid ? seen : cur.valid) - 8 * hh;
+        asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (!partial && 16 * kk + 16 <= cur.valid) continue;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (16 * kk + i >= most) sc[kk >> 1][8 * (kk & 1) + i] = -INFINITY;
+        }
       }
-      stage_tile<T>(tile_k(), tile_v(), src.Tp, klane, vlane, lds + ((t + 1 - t0) & 1) * 32 * kBlock, wave);
-    }
-    if (!busy) continue;
-    const v8* kf = reinterpret_cast<const v8*>(buf) + lane;
-    const v8* vf = reinterpret_cast<const v8*>(buf + 16 * kBlock) + lane;
-    f32x16 sc[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
-#pragma unroll
-      for (int st = 0; st < 8; ++st) sc[kb] = Mma<T>::mul(kf[(kb * 8 + st) * 64], q[st], sc[kb]);
-    }
-    const bool partial = OWN && key0 + valid > it.open, masked = valid < kTile || partial;
-    if (masked) {
-      const int64_t seen = lim - key0;
-      const int most = seen < valid ? (int)(seen < 0 ? 0 : seen) : valid;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      v8 p[4];
+      const float sum = probs<T>(sc, a.c, w.mx == -INFINITY ? 0.0f : w.mx, p);
+      settle<T>(w, sc, a.c, sum, p);
+      if (masked) {
+        masked_pv<T, OWN>(w, cur, partial, vt, vpiece, p);
+      } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7) >= most) sc[kb][i] = -INFINITY;
-    }
-    float top = sc[0][0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, sc[i >> 4][i & 15]);
-    top *= a.c;
-    if (__any(top > mx + kSlack)) {  // as in stream_item
-      const float m2 = fmaxf(mx, over_groups_max(top, 32));
-      const float f = m2 == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m2);
-      mx = m2;
-      sum *= f;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) o[d] *= f;
-    }
-    const float ms = mx == -INFINITY ? 0.0f : mx;
-    v8 p[4];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float e = __builtin_amdgcn_exp2f(sc[i >> 4][i & 15] * a.c - ms);
-      sum += e;
-      p[i >> 3][i & 7] = (T)e;  // rounded to the pool's type; the sum is of fp32 values
-    }
-    if (!masked) {
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) o[d] = Mma<T>::mul(vf[(d * 4 + kk) * 64], p[kk], o[d]);
-    } else {
-      bool odd = false;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          v8 x = drop_behind(vf[(d * 4 + kk) * 64], 16 * kk + 8 * hh, valid);
-          if (partial) odd |= drop_odd<T>(x);  // as in stream_item
-          o[d] = Mma<T>::mul(x, p[kk], o[d]);
-        }
-      if (__any(odd)) {
-#pragma unroll 1
-        for (int key = 0; key < valid; ++key) {
-          float e = pick<T>(p[0], key & 7);
-#pragma unroll
-          for (int kk = 1; kk < 4; ++kk) e = key >> 4 == kk ? pick<T>(p[kk], key & 7) : e;
-          e = __shfl(e, n + 32 * ((key >> 3) & 1), 64);
-          const bool sees = key0 + key < lim;
-          int tp = src.Tp;
-          asm volatile("" : "+s"(tp));
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const int d = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hh + (i & 3);
-            const float x = (float)vb[d * (int64_t)tp + key];
-            if (sees && !__builtin_isfinite(x)) o[i >> 4][i & 15] += e * x;
-            if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
-          }
-        }
+          w.o[i & 3] = Mma<T>::mul(*reinterpret_cast<const v8*>(vt + vpiece[i >> 2] + (i & 3) * 4 * kBlock), p[i >> 2],
+                                   w.o[i & 3]);
+        ahead_of_products();
       }
     }
   }
+  float sum = over_groups_sum(w.sum, 32);
+  if constexpr (WK == 2) {  // the two halves of the waves join through LDS
+    float* const at = reinterpret_cast<float*>(lds) + wr * 66 * 64 + lane;
+    __syncthreads();
+    if (wk == 1) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) at[i * 64] = w.o[i >> 4][i & 15];
+      at[64 * 64] = w.mx;
+      at[65 * 64] = sum;
+    }
+    __syncthreads();
+    if (wk == 1) return;
+    const float m2 = at[64 * 64], l2 = at[65 * 64];
+    const float top = fmaxf(w.mx, m2), ms = top == -INFINITY ? 0.0f : top;
+    const float x = __builtin_amdgcn_exp2f(w.mx - ms), y = __builtin_amdgcn_exp2f(m2 - ms);
+    w.mx = top;
+    sum = sum * x + l2 * y;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) w.o[i >> 4][i & 15] = w.o[i >> 4][i & 15] * x + at[i * 64] * y;
+  }
   if (m >= it.m1) return;
-  sum = over_groups_sum(sum, 32);
   T* dst = nullptr;
-  const float inv = row_out<T>(a, it, m, mx, sum, hh == 0, &dst);
+  const float inv = row_out<T>(a, it, m, w.mx, sum, hh == 0, &dst);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     f32x4 x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = o[i >> 2][4 * (i & 3) + e];
+    for (int e = 0; e < 4; ++e) x[e] = w.o[i >> 2][4 * (i & 3) + e];
     put4<T>(a, it, m, 32 * (i >> 2) + 8 * (i & 3) + 4 * hh, x, inv, dst);
   }
 }
 
-constexpr int kStreamRows = 16, kTileRows = 128;  // rows of a work item
 
-// The prefix's work items first, dealt so that the row blocks of one (key head, split) run on one
-// XCD and share its L2; then every sequence's own pages.  PT, OT: whether the prefix and the own pages
-// go by tiles.
-template <typename T, bool PT, bool OT>
-__global__ __launch_bounds__(256, 2) void attend_shared_kernel(SharedArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[PT || OT ? 64 * kBlock : 2 * 34 * 64 * 4];
-  int bid = blockIdx.x;
+// The prefix's work items first, dealt so that the row blocks of one (key head, split) run one after
+// another on one XCD and share its L2; then every sequence's own pages.  PK, OK: how the prefix and the
+// own pages go (0: streaming, else tiles a round).
+template <typename T, int PK, int OK>
+__global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[PK || OK ? kTileLds : kWaves / 2 * 34 * 64 * 4];
   Item it;
-  if (bid < a.pre_grid) {
-    constexpr int R = PT ? kTileRows : kStreamRows;
-    const int idx = bid >> 3, pair = (idx / a.pre_rb) * 8 + (bid & 7), rb = idx % a.pre_rb;
+  if ((int)blockIdx.x < a.pre_grid) {
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    constexpr int R = kind_rows(PK);
+    const int pair = at / a.pre_rb * 8 + xcd, rb = at % a.pre_rb;
     if (pair >= a.heads * a.pre_splits) return;
     it.h = pair % a.heads;
     it.split = it.part = pair / a.heads;
@@ -770,12 +917,17 @@ __global__ __launch_bounds__(256, 2) void attend_shared_kernel(SharedArgs a) {
     it.n_keys = it.open = a.pre_tokens;
     it.first_lim = 0;
     it.causal = false;
-    if constexpr (PT) tile_item<T, false>(a, a.pre, it, lds);
-    else stream_item<T, false>(a, a.pre, it, reinterpret_cast<float*>(lds));
+    if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
+    else stream_item<T, false>(a, a.pre, it, kWaves, reinterpret_cast<float*>(lds));
     return;
   }
-  constexpr int R = OT ? kTileRows : kStreamRows;
-  bid -= a.pre_grid;
+  constexpr int R = kind_rows(OK);
+  // a workgroup that streams takes as many items as its waves make
+  const int waves = OK ? kWaves : a.own_waves;
+  int bid = ((int)blockIdx.x - a.pre_grid) * (kWaves / waves) +
+            __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / waves;
+  const bool none = bid >= a.own_items;
+  if (none) bid = 0;
   it.split = bid % a.own_splits;
   bid /= a.own_splits;
   const int rb = bid % a.own_rb;
@@ -786,6 +938,7 @@ __global__ __launch_bounds__(256, 2) void attend_shared_kernel(SharedArgs a) {
   it.part = a.pre_splits + it.split;
   it.m0 = b * per + rb * R;
   it.m1 = it.m0 + R < (b + 1) * per ? it.m0 + R : (b + 1) * per;
+  if (none) it.m1 = it.m0;
   it.list = a.tables + b * a.table_st;
   it.n_list = a.width;
   it.causal = a.causal;
@@ -795,46 +948,62 @@ __global__ __launch_bounds__(256, 2) void attend_shared_kernel(SharedArgs a) {
   it.first_lim = length - fresh + 1;
   it.n_keys = a.causal && it.first_lim + l1 < length ? it.first_lim + l1 : length;
   if (it.n_keys > cap) it.n_keys = cap;
-  if (it.n_keys < 0 || l0 >= fresh) it.n_keys = 0;  // no row of the item is a new token
+  if (it.n_keys < 0 || l0 >= fresh || none) it.n_keys = 0;  // no row of the item is a new token
   it.open = a.causal ? it.first_lim + l0 : it.n_keys;
-  if constexpr (OT) tile_item<T, true>(a, a.own, it, lds);
-  else stream_item<T, true>(a, a.own, it, reinterpret_cast<float*>(lds));
+  if constexpr (OK) tile_item<T, OK, true>(a, a.own, it, lds);
+  else stream_item<T, true>(a, a.own, it, waves, reinterpret_cast<float*>(lds));
 }
 
-// One wave per (row, key head): the parts' weights, then their outputs, a lane two channels.
+// One wave per (row, key head).  Lane p weighs part p (64 parts at a time); then each half of the wave
+// adds every other part, a lane four channels, with four loads in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void merge_kernel(SharedArgs a, int n_parts) {
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, half = lane >> 5, c = 4 * (lane & 31);
   if (unit >= (int64_t)a.heads * a.M) return;
   const int h = (int)(unit % a.heads), m = (int)(unit / a.heads);
-  const int gh = m % a.group, bl = m / a.group, l = bl % a.rows, b = bl / a.rows;
-  int fresh = a.rows;
-  if (a.new_lens != nullptr) fresh = a.new_lens[b];
+  int b, l, gh;
+  row_of(a, m, b, l, gh);
   const int64_t at = (int64_t)h * a.M + m, step = (int64_t)a.heads * a.M;
-  float x = 0.0f, y = 0.0f, total = 0.0f;
-  if (l < fresh) {
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  float total = 0.0f;
+  if (l < fresh_rows(a, b)) {
     float top = -INFINITY;
     for (int p = lane; p < n_parts; p += 64) top = fmaxf(top, a.part_ml[at + p * step].x);
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+    top = over_groups_max(top, 1);
     if (top == -INFINITY) top = 0.0f;
-    for (int p = 0; p < n_parts; ++p) {
-      const float2 ml = a.part_ml[at + p * step];
-      const float s = __builtin_amdgcn_exp2f(ml.x - top);
-      const float2 o = *reinterpret_cast<const float2*>(a.part_o + (at + p * step) * kHeadDim + 2 * lane);
-      total += s * ml.y;
-      x += s * o.x;
-      y += s * o.y;
+    for (int p0 = 0; p0 < n_parts; p0 += 64) {
+      const int n = n_parts - p0 < 64 ? n_parts - p0 : 64;
+      float w = 0.0f;
+      if (lane < n) {
+        const float2 ml = a.part_ml[at + (p0 + lane) * step];
+        w = __builtin_amdgcn_exp2f(ml.x - top);
+        total += w * ml.y;
+      }
+      const float* part = a.part_o + (at + p0 * step) * kHeadDim + c;
+      // all lanes make every round (a lane that left could not be asked for its weight)
+#pragma unroll 1
+      for (int p = 0; p < n; p += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const int mine = p + i + half;
+          const float x = __shfl(w, mine & 63, 64);
+          const f32x4 v = *reinterpret_cast<const f32x4*>(part + (mine < n ? mine : 0) * step * kHeadDim);
+          if (mine < n) o += x * v;
+        }
+      }
     }
+    total = over_groups_sum(total, 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32, 64);
   }
   const bool any = total != 0.0f;  // a row that sees no key is zero (NaN sums are not zero)
-  typedef T t2 __attribute__((ext_vector_type(2)));
-  t2 r;
-  r[0] = any ? (T)(x / total) : (T)0.0f;
-  r[1] = any ? (T)(y / total) : (T)0.0f;
-  T* o = static_cast<T*>(a.out) + b * a.o_sb + l * a.o_st + (int64_t)(h * a.group + gh) * a.o_sh;
-  *reinterpret_cast<t2*>(o + 2 * lane) = r;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = any ? (T)(o[i] / total) : (T)0.0f;
+  T* dst = static_cast<T*>(a.out) + b * a.o_sb + l * a.o_st + (int64_t)(h * a.group + gh) * a.o_sh;
+  if (half == 0) *reinterpret_cast<t4*>(dst + c) = r;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -888,10 +1057,69 @@ int common_errors(const char* fn, int dtype, int head_dim, int batch, int rows, 
 
 // The launch of an attention: whether each kind of work item goes by tiles, and the splits.
 struct SharedPlan {
-  bool pre_tiles, own_tiles;
-  int pre_rb, pre_splits, pre_grid, own_rb, own_splits, own_grid, parts;
+  int pre_kind, own_kind;
+  int pre_rb, pre_splits, pre_grid, own_rb, own_splits, own_items, own_waves, own_grid, parts;
   int64_t bytes;
 };
+
+// Key splits, and waves of a streaming item, by what they are estimated to take (microseconds, as
+// measured on MI355X).  A workgroup has a CU to itself, so what counts is rounds of workgroups.  A
+// workgroup takes kFixed to start and end (7.5 us with two steps); a tile of 256 rows 1.7 us with up to
+// two thirds of the CUs busy and 2.2 with all (the clock follows the power), two tiles of 128 rows 2.3; a
+// streaming CU reads 38 GB/s (64 keys in 0.86 us), and the whole chip 4.6 TB/s.  Every part costs its
+// partial results and the merge.
+void choose_splits(const skv_attend_shared_desc* d, int64_t M, int64_t cu, int64_t pre_items, int64_t pre_tiles,
+                   int64_t own_items, int64_t own_tiles, SharedPlan* p) {
+  constexpr double kFixed = 7.0, kBytes = 4.6e6, kMerge = 5.0, kTileBytes = 32768.0;
+  auto tile_cost = [](int kind, double busy) {
+    const double over = (busy < 1.0 ? busy : 1.0) - 0.65;
+    return kind == 0 ? 0.86 : kind == 2 ? 1.15 : 1.7 + (over > 0 ? 1.4 * over : 0.0);
+  };
+  // tables are as wide as their longest sequence gets: the average one holds half of that
+  const double mean = 0.5 * own_tiles, longer = 0.75 * own_tiles;
+  const double own_bytes = mean * own_items * kTileBytes;
+  const double stream = ((double)pre_tiles * d->kv_heads * kTileBytes + own_bytes) / kBytes + kFixed;
+  // short sequences share a workgroup where there is more than one a CU: at most 4 steps a wave
+  int waves = kWaves;
+  if (p->own_kind == 0 && own_items > cu)
+    while (waves > 1 && own_tiles <= waves) waves >>= 1;
+  double best = 1e30;
+  p->pre_splits = pre_tiles > 0, p->own_splits = own_tiles > 0, p->own_waves = waves;
+  for (int os = 1; os <= (waves == kWaves && own_tiles > 1 ? 32 : 1); os *= 2) {
+    const int64_t n_own = own_tiles ? (own_items * os * waves + kWaves - 1) / kWaves : 0;
+    // the prefix's workgroups fill what the own ones leave of a round or two, or a part of a round
+    for (int f = 0; f < (pre_tiles ? 6 : 1); ++f) {
+      int64_t ps = 0;
+      if (pre_tiles) {
+        const int64_t room = f == 0 ? cu - n_own : f == 1 ? 2 * cu - n_own : cu * (f - 1) / 4;
+        ps = room / pre_items;
+        ps = ps < 1 ? 1 : ps > pre_tiles ? pre_tiles : ps > 256 ? 256 : ps;
+      }
+      const int64_t n_pre = pre_items * ps, full = n_pre / cu, part = n_pre % cu;
+      const double busy = (double)(full ? cu : part) / cu;
+      const double dp = ps ? kFixed + (double)((pre_tiles + ps - 1) / ps) * tile_cost(p->pre_kind, busy) : 0.0;
+      const double dn = kFixed + longer / os * tile_cost(p->own_kind, (double)n_own / cu) * kWaves / waves;
+      double t;
+      if (n_pre + n_own <= cu) {
+        t = n_own && dn > dp ? dn : dp;
+      } else {
+        const double rounds = (double)(full + (part > 0)) * dp;
+        const double hidden = part ? (double)(cu - part) * dp / dn : 0.0;  // own workgroups beside the last round
+        const double left = n_own > hidden ? n_own - hidden : 0.0;
+        double tail = left / cu * dn;
+        if (tail < left / (n_own ? n_own : 1) * own_bytes / kBytes) tail = left / n_own * own_bytes / kBytes;
+        t = rounds + (left > 0 ? tail + 0.5 * dn : 0.0);
+      }
+      if (t < stream) t = stream;
+      if (ps + os * (own_tiles > 0) > 1) t += kMerge + (double)(ps + os) * M * d->kv_heads * 1040 / kBytes;
+      if (t < best) {
+        best = t;
+        p->pre_splits = (int)ps;
+        p->own_splits = own_tiles ? os : 0;
+      }
+    }
+  }
+}
 
 int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) {
   const int group = d->q_heads / d->kv_heads;
@@ -902,9 +1130,9 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
   }
   *p = SharedPlan{};
   const bool pre = d->prefix_tokens > 0, own = d->table_width > 0;
-  p->own_tiles = per > kStreamRows;
-  p->pre_tiles = pre ? M > kStreamRows : p->own_tiles;
-  const int pre_rows = p->pre_tiles ? kTileRows : kStreamRows, own_rows = p->own_tiles ? kTileRows : kStreamRows;
+  p->own_kind = kind_of(per);
+  p->pre_kind = pre ? kind_of(M) : p->own_kind;
+  const int pre_rows = kind_rows(p->pre_kind), own_rows = kind_rows(p->own_kind);
   const int64_t cu = cu_count();
   auto tiles = [](int64_t tokens, int64_t page) {
     return tokens / page * ((page + kTile - 1) / kTile) + (tokens % page + kTile - 1) / kTile;
@@ -915,23 +1143,17 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
   p->own_rb = own ? (int)((per + own_rows - 1) / own_rows) : 0;
   const int64_t pre_items = (int64_t)p->pre_rb * d->kv_heads;
   const int64_t own_items = (int64_t)p->own_rb * d->kv_heads * d->batch;
-  int64_t share = (pre_items * pre_tiles + own_items * own_tiles + 2 * cu - 1) / (2 * cu);
-  if (share < 8) share = 8;
-  auto splits = [&](int64_t n) -> int {
-    const int64_t s = (n + share - 1) / share;
-    return (int)(s < 1 ? 1 : s > 1024 ? 1024 : s);
-  };
-  p->pre_splits = pre ? splits(pre_tiles) : 0;
-  p->own_splits = own ? splits(own_tiles) : 0;
+  choose_splits(d, M, cu, pre_items, pre_tiles, own_items, own_tiles, p);
   p->parts = p->pre_splits + p->own_splits;
-  const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits;
-  const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, own_grid = own_items * p->own_splits;
-  if (pre_grid + own_grid >= ((int64_t)1 << 31)) {
+  const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits, each = p->own_kind ? 1 : kWaves / p->own_waves;
+  const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, all_own = own_items * p->own_splits;
+  if (pre_grid + all_own >= ((int64_t)1 << 31)) {
     set_error("%s: too many work items", fn);
     return SKV_E_ARG;
   }
   p->pre_grid = (int)pre_grid;
-  p->own_grid = (int)own_grid;
+  p->own_items = (int)all_own;
+  p->own_grid = (int)((all_own + each - 1) / each);
   p->bytes = p->parts > 1 ? (int64_t)p->parts * d->kv_heads * M * (kHeadDim * 4 + 8) : 0;
   return SKV_OK;
 }
@@ -973,10 +1195,13 @@ int check_shared(const char* fn, const skv_attend_shared_desc* d) {
 
 template <typename T>
 void launch_shared(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.pre_grid + p.own_grid)), block(256);
-  if (!p.pre_tiles) hipLaunchKernelGGL((attend_shared_kernel<T, false, false>), grid, block, 0, s, a);
-  else if (!p.own_tiles) hipLaunchKernelGGL((attend_shared_kernel<T, true, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((attend_shared_kernel<T, true, true>), grid, block, 0, s, a);
+  const dim3 grid((unsigned)(p.pre_grid + p.own_grid)), block(64 * kWaves);
+  auto launch = [&](void (*kernel)(SharedArgs)) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a); };
+  if (p.pre_kind == 0) launch(attend_shared_kernel<T, 0, 0>);
+  else if (p.pre_kind == 2) p.own_kind == 0 ? launch(attend_shared_kernel<T, 2, 0>) : launch(attend_shared_kernel<T, 2, 2>);
+  else if (p.own_kind == 0) launch(attend_shared_kernel<T, 1, 0>);
+  else if (p.own_kind == 2) launch(attend_shared_kernel<T, 1, 2>);
+  else launch(attend_shared_kernel<T, 1, 1>);
 }
 
 }  // namespace
@@ -1120,11 +1345,12 @@ extern "C" int skv_attend_shared(const skv_attend_shared_desc* d, skv_stream_t s
   a.M = d->batch * d->rows * a.group;
   a.pre_rb = p.pre_rb, a.pre_splits = p.pre_splits, a.pre_grid = p.pre_grid;
   a.own_rb = p.own_rb, a.own_splits = p.own_splits;
+  a.own_items = p.own_items, a.own_waves = p.own_waves;
   a.direct = p.parts == 1;
   a.part_o = static_cast<float*>(d->workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)p.parts * a.heads * a.M * kHeadDim);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p.pre_grid + p.own_grid > 0) {
+  if (p.parts > 0) {
     if (d->dtype == SKV_BF16) launch_shared<bf16>(a, p, s);
     else launch_shared<f16>(a, p, s);
     st = launched(fn);
