@@ -29,8 +29,8 @@ import torch
 
 from . import _lib, kernels
 from .cache import SlotKVCache
-from .qknorm import (HEAD_DIM, check_heads, check_positions, check_tables, head_norm_spec, launch,
-                     same_device, strides)
+from .qknorm import (HEAD_DIM, check_heads, check_positions, check_tables, empty_as, head_norm_spec,
+                     launch, same_device, strides)
 
 _HALVES = (torch.bfloat16, torch.float16)
 
@@ -45,7 +45,7 @@ def _check_pools(what: str, kpool: torch.Tensor, vpool: torch.Tensor, page_token
         raise ValueError(f"{what}pools must be K [pages, 1, H, Tp, 128] / V [pages, 1, H, 128, Tp], got "
                          f"{tuple(kpool.shape)}")
     n, _, h = kpool.shape[:3]
-    if tuple(kpool.shape[3:]) != (tp, HEAD_DIM) or tuple(vpool.shape) != (n, 1, h, HEAD_DIM, tp):
+    if kpool.shape != (n, 1, h, tp, HEAD_DIM) or vpool.shape != (n, 1, h, HEAD_DIM, tp):
         raise ValueError(f"{what}pool shapes {tuple(kpool.shape)} / {tuple(vpool.shape)} do not match "
                          f"page_tokens={page_tokens} (Tp = {tp})")
     if kpool.dtype != dtype or vpool.dtype != dtype:
@@ -58,7 +58,7 @@ def _check_pools(what: str, kpool: torch.Tensor, vpool: torch.Tensor, page_token
 
 
 def _int32_vector(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
-    if t.dtype != torch.int32 or tuple(t.shape) != (n,):
+    if t.dtype != torch.int32 or t.shape != (n,):
         raise ValueError(f"{name} must be int32 [{n}], got {t.dtype} {tuple(t.shape)}")
     if n > 1 and t.stride(0) != 1:
         raise ValueError(f"{name} must be contiguous")
@@ -136,7 +136,7 @@ def append_pages(
         if q.dtype != k.dtype or q.shape[:2] != k.shape[:2] or q.shape[2] == 0:
             raise ValueError(f"q must share k's dtype, batch and length, got {q.dtype} {tuple(q.shape)}")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = empty_as(q)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out must match q's shape and dtype")
         d.q, d.q_out, d.q_heads = q.data_ptr(), out.data_ptr(), q.shape[2]
@@ -160,8 +160,9 @@ def append_pages(
             raise ValueError("positions without cos and sin")
         d.pos_sb, d.pos_st = check_positions(positions, b, l)
         d.positions, d.pos_is_int64 = positions.data_ptr(), positions.dtype == torch.int64
-    same_device(kpool, kpool=kpool, vpool=vpool, k=k, v=v, q=q, out=out, tables=tables, lengths=lengths,
-                new_lens=new_lens, cos=cos, sin=sin, positions=positions, norm_q=wq, norm_k=wk)
+    same_device(("k_pool", "v_pool", "k", "v", "q", "out", "tables", "lengths", "new_lens", "cos", "sin",
+                 "positions", "norm_q", "norm_k"),
+                (kpool, vpool, k, v, q, out, tables, lengths, new_lens, cos, sin, positions, wq, wk))
     if k.numel():
         launch("skv_append_pages", d, k.device)
     return out
@@ -223,19 +224,21 @@ def attend_shared(
     else:
         prefix_pages = None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = empty_as(q)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must match q's shape and dtype")
     d.q, d.out = q.data_ptr(), out.data_ptr()
     d.q_sb, d.q_st, d.q_sh = strides("q", q)
     d.out_sb, d.out_st, d.out_sh = strides("out", out)
-    same_device(kpool, kpool=kpool, vpool=vpool, q=q, out=out, tables=tables, lengths=lengths,
-                new_lens=new_lens, prefix_pages=prefix_pages, prefix_kpool=pk, prefix_vpool=pv)
+    same_device(("k_pool", "v_pool", "q", "out", "tables", "lengths", "new_lens", "prefix_pages",
+                 "prefix k_pool", "prefix v_pool"),
+                (kpool, vpool, q, out, tables, lengths, new_lens, prefix_pages, pk, pv))
     if q.numel() == 0:
         return out
     size = ctypes.c_int64(0)
-    _lib.check("skv_attend_shared_workspace",
-               _lib.load().skv_attend_shared_workspace(ctypes.byref(d), ctypes.byref(size)))
+    status = _lib.load().skv_attend_shared_workspace(ctypes.byref(d), ctypes.byref(size))
+    if status:
+        _lib.check("skv_attend_shared_workspace", status)
     ws = None
     if size.value:
         # a block of this call's own: two graphs captured on one stream may replay side by side

@@ -90,13 +90,24 @@ def check_positions(positions, batch: int, rows: int) -> tuple[int, int]:
     raise ValueError(f"positions must be [{rows}] or [{batch}, {rows}], got {tuple(positions.shape)}")
 
 
-def same_device(first: torch.Tensor, **tensors) -> None:
-    """Every tensor that is given is on the GPU of ``first``."""
-    for name, t in tensors.items():
+def same_device(names: tuple[str, ...], tensors: tuple) -> None:
+    """Every tensor that is given is on the GPU of the first."""
+    device = tensors[0].device
+    if device.type == "cuda":
+        for t in tensors:
+            if t is not None and t.device != device:
+                break
+        else:
+            return
+    for name, t in zip(names, tensors):
         if t is not None:
             kernels._require_cuda(name, t)
-            if t.device != first.device:
-                raise ValueError(f"{name} is on {t.device}, expected {first.device}")
+            if t.device != device:
+                raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def empty_as(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _desc(q, k, wq, wk, cos, sin, positions, meta) -> _lib.QkNormRopeDesc:
@@ -130,8 +141,7 @@ def _set_out(side, x: torch.Tensor) -> None:
 
 
 def _forward(q, k, wq, wk, cos, sin, positions, meta):
-    zq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    zk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    zq, zk = empty_as(q), None if k is None else empty_as(k)
     if q.numel() == 0:
         return zq, zk
     d = _desc(q, k, wq, wk, cos, sin, positions, meta)
@@ -162,8 +172,7 @@ class _QkNormRope(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = empty_as(q), None if k is None else empty_as(k)
         need = ctx.needs_input_grad
         dwq = torch.empty_like(wq) if need[2] else None
         dwk = torch.empty_like(wk) if need[3] else None
@@ -186,8 +195,9 @@ class _QkNormRope(torch.autograd.Function):
                 s.grad_weight, s.grad_weight_dtype = dw.data_ptr(), kernels.dtype_code(dw.dtype)
         if dwq is not None or dwk is not None:
             size = ctypes.c_int64(0)
-            launch_size = _lib.load().skv_qk_norm_rope_grad_workspace(ctypes.byref(d), ctypes.byref(size))
-            _lib.check("skv_qk_norm_rope_grad_workspace", launch_size)
+            status = _lib.load().skv_qk_norm_rope_grad_workspace(ctypes.byref(d), ctypes.byref(size))
+            if status:
+                _lib.check("skv_qk_norm_rope_grad_workspace", status)
             # a block of this call's own: two graphs captured on one stream may replay side by side
             ws = torch.empty(size.value, dtype=torch.uint8, device=q.device)
             d.workspace, d.workspace_bytes = ws.data_ptr(), size.value
@@ -246,9 +256,11 @@ def qk_norm_rope(
     elif cos is not None and not 0 <= position0 <= cos.shape[0] - q.shape[1]:
         raise ValueError(f"positions {position0} .. {position0 + q.shape[1] - 1} do not lie in a table of "
                          f"{cos.shape[0]} rows")
-    same_device(q, q=q, k=k, cos=cos, sin=sin, norm_q=wq, norm_k=wk, positions=positions)
+    same_device(("q", "k", "cos", "sin", "norm_q", "norm_k", "positions"),
+                (q, k, cos, sin, wq, wk, positions))
     meta = (norm_q is not None, eps_q, norm_k is not None, eps_k, position0, bool(interleaved))
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (q, k, wq, wk)):
+    if torch.is_grad_enabled() and (
+            q.requires_grad or (k is not None and k.requires_grad)
+            or (wq is not None and wq.requires_grad) or (wk is not None and wk.requires_grad)):
         return _QkNormRope.apply(q, k, wq, wk, cos, sin, positions, meta)
     return _forward(q, k, wq, wk, cos, sin, positions, meta)
