@@ -49,14 +49,17 @@ struct AppendPagesArgs {
   int v_tiles;                            // per (sequence, head); 0: a wave per token instead
 };
 
-// The page row of a sequence's token `own`: its row in [pages][T], or -1 where there is none.
-__device__ inline int64_t page_of(const Pages& pg, int b, int64_t own, int* off) {
-  if (own < 0) return -1;
+// Where a sequence's token `own` lies: its page (-1 where there is none) and its place in it.
+struct Place {
+  int64_t page;
+  int off;
+};
+__device__ inline Place place_of(const Pages& pg, int b, int64_t own) {
+  if (own < 0) return Place{-1, 0};
   const int64_t p = own / pg.T;
-  if (p >= pg.width) return -1;
-  *off = (int)(own - p * pg.T);
+  if (p >= pg.width) return Place{-1, 0};
   const int id = pg.tables[b * pg.table_st + p];
-  return id < 0 || id >= pg.n_pages ? -1 : id;
+  return Place{id < 0 || id >= pg.n_pages ? -1 : id, (int)(own - p * pg.T)};
 }
 
 // V of one token and head by one wave: a lane's two channels go to two rows of the page.
@@ -68,13 +71,12 @@ __device__ inline void v_token(const AppendPagesArgs& a, int unit) {
   if (b >= a.batch) return;
   const int n = a.pg.fresh(b, a.rows);
   if (row >= n) return;
-  int off = 0;
-  const int64_t page = page_of(a.pg, b, a.pg.first(b, n) + row, &off);
-  if (page < 0) return;
+  const Place at = place_of(a.pg, b, a.pg.first(b, n) + row);
+  if (at.page < 0) return;
   const uint32_t w = *reinterpret_cast<const uint32_t*>(
       static_cast<const T*>(a.v) + b * a.v_sb + row * a.v_st + h * a.v_sh + 2 * lane);
   uint16_t* o = static_cast<uint16_t*>(a.v_pool) +
-                ((page * a.pg.heads + h) * kHeadDim + 2 * lane) * (int64_t)a.pg.Tp + off;
+                ((at.page * a.pg.heads + h) * kHeadDim + 2 * lane) * (int64_t)a.pg.Tp + at.off;
   o[0] = (uint16_t)w;
   o[a.pg.Tp] = (uint16_t)(w >> 16);
 }
@@ -191,9 +193,8 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
     o = static_cast<T*>(a.q_out) + b * a.o_sb + row * a.o_st;
     oh = a.o_sh;
   } else if (token) {
-    int off = 0;
-    const int64_t page = page_of(a.pg, b, own, &off);
-    if (page >= 0) o = static_cast<T*>(a.k_pool) + (page * a.pg.heads * a.pg.Tp + off) * kHeadDim;
+    const Place at = place_of(a.pg, b, own);
+    if (at.page >= 0) o = static_cast<T*>(a.k_pool) + (at.page * a.pg.heads * a.pg.Tp + at.off) * kHeadDim;
     oh = (int64_t)a.pg.Tp * kHeadDim;
   }
   const bool norm = is_q ? a.norm_q : a.norm_k;
@@ -229,6 +230,7 @@ constexpr int kWaves = 8;    // of a workgroup: one workgroup a CU, two waves a 
 constexpr int kind_rows(int kind) { return kind == 0 ? 16 : 32 * kWaves / kind; }
 constexpr int kind_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 128 ? 2 : 1; }
 constexpr int kStep = 32;    // keys of a streaming step
+constexpr int kCompact = 1024;  // sequences whose padding rows a prefix by tiles leaves out
 constexpr float kSlack = 8;  // the running maximum may lag the true one by 2^8 (see below)
 
 struct Source {
@@ -263,6 +265,7 @@ struct SharedArgs {
 struct Item {
   const int32_t* list;  // page numbers
   int n_list, h, m0, m1, n_split, split, part;
+  const int* tokens;  // rows count new tokens only: exclusive sums of new_lens in LDS (NULL: all rows)
   int64_t n_keys;     // keys that some row sees
   int64_t open;       // keys that every row sees
   int64_t first_lim;  // keys that row 0 of the sequence sees (causal; each next row one more)
@@ -378,6 +381,18 @@ __device__ inline void row_of(const SharedArgs& a, int m, int& b, int& l, int& g
   const int bl = m / a.group;
   l = bl % a.rows;
   b = bl / a.rows;
+}
+
+// Row m of a work item that counts new tokens only, among all rows.
+__device__ inline int all_rows(const SharedArgs& a, const Item& it, int m) {
+  if (it.tokens == nullptr) return m;
+  const int tk = m / a.group;
+  int lo = 0, hi = a.batch;  // the last sequence that begins at or before token tk
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (it.tokens[mid] <= tk ? lo : hi) = mid;
+  }
+  return (lo * a.rows + tk - it.tokens[lo]) * a.group + m % a.group;
 }
 
 __device__ inline int fresh_rows(const SharedArgs& a, int b) {
@@ -587,9 +602,8 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
 // different banks.  Row i of a K operand is key 16 (i / 16) + 8 ((i / 4) % 2) + 4 ((i / 8) % 2) + i % 4
 // of its 32: the 16 scores of lane (n, hh) are then row n's keys 8 hh .. 8 hh + 7 and 16 + 8 hh .. + 7.
 //
-// Two waves a SIMD: one's softmax runs under the other's products.
 constexpr int kBlock = 1024;  // bytes that a wave's direct load fills
-constexpr int kRing = 4;       // tiles in LDS: one in use, three on their way
+constexpr int kRing = 4;  // tiles in LDS
 constexpr int kTileLds = kRing * 32 * kBlock;
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -759,10 +773,11 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
   constexpr int kRows = kWaves / WK;  // waves side by side
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hh = lane >> 5, wr = wave % kRows, wk = wave / kRows;
-  const int m = it.m0 + 32 * wr + n;
   const bool busy = it.m0 + 32 * wr < it.m1;  // the wave has rows at all
+  const bool mine = it.m0 + 32 * wr + n < it.m1;
+  const int m = all_rows(a, it, mine ? it.m0 + 32 * wr + n : it.m0);
   int b, l, gh;
-  row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
+  row_of(a, m, b, l, gh);
   const int lim = (int)(OWN && it.causal ? it.first_lim + l : it.n_keys);
   TileState<T> w;
   {
@@ -882,7 +897,7 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
 #pragma unroll
     for (int i = 0; i < 64; ++i) w.o[i >> 4][i & 15] = w.o[i >> 4][i & 15] * x + at[i * 64] * y;
   }
-  if (m >= it.m1) return;
+  if (!mine) return;
   T* dst = nullptr;
   const float inv = row_out<T>(a, it, m, w.mx, sum, hh == 0, &dst);
 #pragma unroll
@@ -901,6 +916,7 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
 template <typename T, int PK, int OK>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[PK || OK ? kTileLds : kWaves / 2 * 34 * 64 * 4];
+  __shared__ int tokens[PK ? kCompact + 1 : 1];
   Item it;
   if ((int)blockIdx.x < a.pre_grid) {
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
@@ -910,8 +926,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
     it.h = pair % a.heads;
     it.split = it.part = pair / a.heads;
     it.n_split = a.pre_splits;
+    int rows = a.M;
+    it.tokens = nullptr;
+    if constexpr (PK) {
+      // a padded batch: its new tokens close up, so that the prefix meets rows that count
+      if (a.new_lens != nullptr && a.batch <= kCompact && !a.direct) {
+        if (threadIdx.x < 64) {
+          int sum = 0;
+          for (int b0 = 0; b0 < a.batch; b0 += 64) {
+            const int i = b0 + threadIdx.x, n = i < a.batch ? fresh_rows(a, i) : 0;
+            int upto = n;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+              const int other = __shfl_up(upto, d, 64);
+              if ((int)threadIdx.x >= d) upto += other;
+            }
+            if (i < a.batch) tokens[i] = sum + upto - n;
+            sum += __shfl(upto, 63, 64);
+          }
+          if (threadIdx.x == 0) tokens[a.batch] = sum;
+        }
+        __syncthreads();
+        it.tokens = tokens;
+        rows = __builtin_amdgcn_readfirstlane(tokens[a.batch]) * a.group;
+        if (rb * R >= rows) return;
+      }
+    }
     it.m0 = rb * R;
-    it.m1 = it.m0 + R < a.M ? it.m0 + R : a.M;
+    it.m1 = it.m0 + R < rows ? it.m0 + R : rows;
     it.list = a.pre_pages;
     it.n_list = (int)((a.pre_tokens + a.pre.T - 1) / a.pre.T);
     it.n_keys = it.open = a.pre_tokens;
@@ -939,6 +981,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
   it.m0 = b * per + rb * R;
   it.m1 = it.m0 + R < (b + 1) * per ? it.m0 + R : (b + 1) * per;
   if (none) it.m1 = it.m0;
+  it.tokens = nullptr;
   it.list = a.tables + b * a.table_st;
   it.n_list = a.width;
   it.causal = a.causal;
@@ -1143,7 +1186,9 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
   p->own_rb = own ? (int)((per + own_rows - 1) / own_rows) : 0;
   const int64_t pre_items = (int64_t)p->pre_rb * d->kv_heads;
   const int64_t own_items = (int64_t)p->own_rb * d->kv_heads * d->batch;
-  choose_splits(d, M, cu, pre_items, pre_tiles, own_items, own_tiles, p);
+  // of a padded batch's row blocks about half hold tokens
+  const int64_t busy_rb = d->new_lens && p->pre_kind ? (M / 2 + pre_rows) / pre_rows : p->pre_rb;
+  choose_splits(d, M, cu, busy_rb < p->pre_rb ? busy_rb * d->kv_heads : pre_items, pre_tiles, own_items, own_tiles, p);
   p->parts = p->pre_splits + p->own_splits;
   const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits, each = p->own_kind ? 1 : kWaves / p->own_waves;
   const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, all_own = own_items * p->own_splits;

@@ -156,26 +156,29 @@ __global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(QkArgs a) {
   }
 }
 
-// grid 2 (q, k), block 1024: the weight gradient from the workgroups' partials, in a fixed order.
+// grid (4, 2): 32 channels of q's or k's weight gradient from the workgroups' partials, in a fixed order.
 __global__ __launch_bounds__(1024) void qk_norm_dw_kernel(QkArgs a, int n_groups_k) {
-  __shared__ float part[32][kHeadDim];
-  const QkSide& s = blockIdx.x == 0 ? a.q : a.k;
+  __shared__ float part[128][33];
+  const QkSide& s = blockIdx.y == 0 ? a.q : a.k;
   if (s.dw == nullptr) return;
-  const int n = blockIdx.x == 0 ? a.n_groups_q : n_groups_k;
-  const int c = 4 * (threadIdx.x & 31), j = threadIdx.x >> 5;
+  const int n = blockIdx.y == 0 ? a.n_groups_q : n_groups_k;
+  const int c = 4 * (threadIdx.x & 7), j = threadIdx.x >> 3, c0 = 32 * blockIdx.x;
   f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int i = j; i < n; i += 32)
-    t += *reinterpret_cast<const f32x4*>(s.dw_part + (int64_t)i * kHeadDim + c);
-  *reinterpret_cast<f32x4*>(&part[j][c]) = t;
-  __syncthreads();
-  if (threadIdx.x < kHeadDim) {
-    float sum = 0.0f;
+  for (int i = j; i < n; i += 128)
+    t += *reinterpret_cast<const f32x4*>(s.dw_part + (int64_t)i * kHeadDim + c0 + c);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) sum += part[i][threadIdx.x];
-    if (s.dw_dtype == SKV_F32) static_cast<float*>(s.dw)[threadIdx.x] = sum;
-    else if (s.dw_dtype == SKV_BF16) static_cast<bf16*>(s.dw)[threadIdx.x] = (bf16)sum;
-    else static_cast<f16*>(s.dw)[threadIdx.x] = (f16)sum;
+  for (int i = 0; i < 4; ++i) part[j][c + i] = t[i];
+  __syncthreads();
+  // 32 threads a channel, four rows each, then across them
+  const int ch = threadIdx.x >> 5, k = threadIdx.x & 31;
+  float sum = part[k][ch] + part[k + 32][ch] + part[k + 64][ch] + part[k + 96][ch];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d, 64);
+  if (k == 0) {
+    if (s.dw_dtype == SKV_F32) static_cast<float*>(s.dw)[c0 + ch] = sum;
+    else if (s.dw_dtype == SKV_BF16) static_cast<bf16*>(s.dw)[c0 + ch] = (bf16)sum;
+    else static_cast<f16*>(s.dw)[c0 + ch] = (f16)sum;
   }
 }
 
@@ -386,7 +389,7 @@ extern "C" int skv_qk_norm_rope_grad(const skv_qk_norm_rope_desc* d, skv_stream_
     if (e != SKV_OK) return e;
   }
   if (a.q.dw || a.k.dw) {
-    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2), dim3(1024), 0, s, a, nk);
+    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(4, 2), dim3(1024), 0, s, a, nk);
     return launched(fn);
   }
   return SKV_OK;
