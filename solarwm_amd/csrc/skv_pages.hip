@@ -266,8 +266,8 @@ struct Item {
   const int32_t* list;  // page numbers
   int n_list, h, m0, m1, n_split, split, part;
   const int* tokens;  // rows count new tokens only: exclusive sums of new_lens in LDS (NULL: all rows)
-  int64_t n_keys;     // keys that some row sees
-  int64_t open;       // keys that every row sees
+  int n_keys;         // keys that some row sees (below 2^31)
+  int open;           // keys that every row sees
   int64_t first_lim;  // keys that row 0 of the sequence sees (causal; each next row one more)
   bool causal;
 };
@@ -352,28 +352,37 @@ __device__ inline float marked(int kind) { return kind == 2 ? __builtin_nanf("")
 struct PageWalk {
   const int32_t* list;
   int n, base, ids;
-  __device__ void start(const int32_t* l, int count, int page) {
+  __device__ void start(const int32_t* l, int count, int page) {  // then landed(), before the first get()
     list = l;
     n = count;
-    fill(page);
+    load(page);
   }
-  __device__ void fill(int page) {
+  __device__ void load(int page) {
     base = page;
     const int i = page + (int)(threadIdx.x & 63);
     ids = i < n ? list[i] : -1;
-    // waited for here, not wherever the paths meet again: there it would drain the tiles under way
-    asm volatile("" : "+v"(ids));
   }
+  // The load's wait stands here, not wherever the paths meet again: there it would drain the tiles under way.
+  __device__ void landed() { asm volatile("" : "+v"(ids)); }
   __device__ int get(int page) {
-    if (page - base >= 64) fill(page);
+    if (page - base >= 64) {
+      load(page);
+      landed();
+    }
     return __builtin_amdgcn_readlane(ids, page - base);
   }
 };
 
 // The steps of `step` keys that n_keys take: whole pages, then what the last page holds.
-__device__ inline int steps_of(const Source& src, int64_t n_keys, int step, int per_page) {
-  const int64_t full = n_keys / src.T;
-  return (int)(full * per_page) + ((int)(n_keys - full * src.T) + step - 1) / step;
+__device__ inline int steps_of(const Source& src, int n_keys, int step, int per_page) {
+  const int full = n_keys / src.T;
+  return full * per_page + (n_keys - full * src.T + step - 1) / step;
+}
+
+// Where share `i` of `n` begins in `all` steps: shares differ by one step at most.
+__device__ inline int share_of(int all, int i, int n) {
+  const int each = all / n, more = all - each * n;
+  return i * each + (i < more ? i : more);
 }
 
 __device__ inline void row_of(const SharedArgs& a, int m, int& b, int& l, int& gh) {
@@ -441,10 +450,17 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
   typedef typename Mma<T>::v8 v8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave & (waves - 1), n = lane & 15, g = lane >> 4;
+  const int per_page = (src.T + kStep - 1) / kStep;
+  const int n_steps = steps_of(src, it.n_keys, kStep, per_page);
+  const int share = it.n_split * waves, mine = it.split * waves + wk;
+  const int s0 = share_of(n_steps, mine, share), s1 = share_of(n_steps, mine + 1, share);
+  PageWalk pages;
+  int page = s0 / per_page, in_page = s0 - page * per_page;
+  if (s0 < s1) pages.start(it.list, it.n_list, page);  // loads while the rows are looked up
   const int m = it.m0 + n;
   int b, l, gh;
   row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
-  const int lim = (int)(OWN && it.causal ? it.first_lim + l : it.n_keys);
+  const int lim = OWN && it.causal ? (int)(it.first_lim + l > 0 ? it.first_lim + l : 0) : it.n_keys;
   v8 q[4];
   {
     const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
@@ -456,17 +472,11 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
 #pragma unroll
   for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float mx = -INFINITY, sum = 0.0f;
-  const int per_page = (src.T + kStep - 1) / kStep;
-  const int n_steps = steps_of(src, it.n_keys, kStep, per_page);
-  const int share = it.n_split * waves, mine = it.split * waves + wk;
-  const int s0 = (int)((int64_t)n_steps * mine / share), s1 = (int)((int64_t)n_steps * (mine + 1) / share);
   if (s0 < s1) {
     const int k_off = ((n >> 2) * 8 + (n & 3)) * kHeadDim + g * 8, v_off = n * src.Tp + g * 8;
     const T* kp = static_cast<const T*>(src.k_pool);
     const T* vp = static_cast<const T*>(src.v_pool);
-    PageWalk pages;
-    int page = s0 / per_page, in_page = s0 - page * per_page;
-    pages.start(it.list, it.n_list, page);
+    pages.landed();
     int id = pages.get(page);
     v8 kf[2][4];
     auto load_k = [&](int id, int at) {
@@ -487,12 +497,12 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
       v8 vf[8];
 #pragma unroll
       for (int d = 0; d < 8; ++d) vf[d] = *reinterpret_cast<const v8*>(vb + d * 16 * (int64_t)src.Tp + v_off);
-      const int64_t key0 = (int64_t)page * src.T + in_page * kStep;
+      const int key0 = page * src.T + in_page * kStep;
       // keys of this step that exist: inside the page, inside the sequence
-      int64_t left = it.n_keys - key0;
+      int left = it.n_keys - key0;
       const int in_tile = src.T - in_page * kStep;
       if (left > in_tile) left = in_tile;
-      const int valid = there ? (left > kStep ? kStep : (int)left) : 0;
+      const int valid = there ? (left > kStep ? kStep : left) : 0;
       f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int st = 0; st < 4; ++st)
@@ -508,7 +518,7 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
       }
       const bool partial = OWN && key0 + valid > it.open;  // some row may not see all of them
       if (valid < kStep || partial) {
-        const int seen = lim - (int)key0, most = seen < valid ? seen : valid;
+        const int seen = lim - key0, most = seen < valid ? seen : valid;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (8 * g + i >= most) sc[i >> 2][i & 3] = -INFINITY;
@@ -609,8 +619,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 // Where a tile lies and what of it exists.
 struct TileAt {
-  int64_t base;  // (page * heads + head), page 0 for one that is not there
-  int64_t key0;  // number of its first key
+  int64_t base;  // elements to its page's rows of the head (K and V alike); page 0 where there is none
+  int key0;      // number of its first key
   int tok0;      // its first token in the page
   int valid;     // keys that exist
 };
@@ -623,6 +633,9 @@ struct TileWalk {
     page = tile / per;
     in_page = tile - page * per;
     pages.start(it.list, it.n_list, page);
+  }
+  __device__ void first() {
+    pages.landed();
     id = pages.get(page);
   }
   __device__ void next() {
@@ -631,15 +644,16 @@ struct TileWalk {
       id = pages.get(++page);
     }
   }
-  __device__ TileAt at(const Source& src, const Item& it, int heads) const {
+  // head_size: elements of a page's rows of one head
+  __device__ TileAt at(const Source& src, const Item& it, int heads, int64_t head_size) const {
     TileAt x;
     const bool there = id >= 0 && id < src.n_pages;
-    x.base = (int64_t)(there ? id : 0) * heads + it.h;
+    x.base = ((int64_t)(there ? id : 0) * heads + it.h) * head_size;
     x.tok0 = in_page * kTile;
-    x.key0 = (int64_t)page * src.T + x.tok0;
-    int64_t left = it.n_keys - x.key0;
+    x.key0 = page * src.T + x.tok0;
+    int left = it.n_keys - x.key0;
     if (left > src.T - x.tok0) left = src.T - x.tok0;
-    x.valid = there ? (left > kTile ? kTile : (int)left) : 0;
+    x.valid = there ? (left > kTile ? kTile : left) : 0;
     return x;
   }
 };
@@ -647,8 +661,8 @@ struct TileWalk {
 // A wave's share of a tile: 8 keys of K and twice 8 channels of V^T.  `lane` and `dst` are its own.
 template <typename T>
 __device__ inline void stage_tile(const Source& src, const TileAt& x, int klane, int vlane, char* dst, int wave) {
-  const T* kt = static_cast<const T*>(src.k_pool) + (x.base * src.Tp + x.tok0) * kHeadDim;
-  const T* vt = static_cast<const T*>(src.v_pool) + x.base * kHeadDim * (int64_t)src.Tp + x.tok0;
+  const T* kt = static_cast<const T*>(src.k_pool) + x.base + x.tok0 * kHeadDim;
+  const T* vt = static_cast<const T*>(src.v_pool) + x.base + x.tok0;
   const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kt, (short)0, 0x7fffffff, 0x00020000);
   const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vt, (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
@@ -773,21 +787,23 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
   constexpr int kRows = kWaves / WK;  // waves side by side
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hh = lane >> 5, wr = wave % kRows, wk = wave / kRows;
+  const int per_page = (src.T + kTile - 1) / kTile;
+  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
+  const int t0 = share_of(n_tiles, it.split, it.n_split), n_own = share_of(n_tiles, it.split + 1, it.n_split) - t0;
+  TileWalk walk;  // at the tile that loads last
+  if (n_own > 0) walk.start(it, per_page, t0);  // the page list loads while the rows are looked up
   const bool busy = it.m0 + 32 * wr < it.m1;  // the wave has rows at all
   const bool mine = it.m0 + 32 * wr + n < it.m1;
   const int m = all_rows(a, it, mine ? it.m0 + 32 * wr + n : it.m0);
   int b, l, gh;
   row_of(a, m, b, l, gh);
-  const int lim = (int)(OWN && it.causal ? it.first_lim + l : it.n_keys);
+  const int lim = OWN && it.causal ? (int)(it.first_lim + l > 0 ? it.first_lim + l : 0) : it.n_keys;
   TileState<T> w;
   {
     const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
                  (int64_t)(it.h * a.group + gh) * a.q_sh + hh * 8;
 #pragma unroll
     for (int st = 0; st < 8; ++st) w.q[st] = *reinterpret_cast<const v8*>(p + st * 16);
-    // the queries' own wait, ahead of the loop's counted ones
-#pragma unroll
-    for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
   }
 #pragma unroll
   for (int d = 0; d < 4; ++d)
@@ -795,10 +811,6 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
     for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
   w.mx = -INFINITY;
   w.sum = 0.0f;
-  const int per_page = (src.T + kTile - 1) / kTile;
-  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
-  const int t0 = (int)((int64_t)n_tiles * it.split / it.n_split);
-  const int n_own = (int)((int64_t)n_tiles * (it.split + 1) / it.n_split) - t0;
   const int key_row = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
   // loads: lane (r, c) of a wave takes row r of its 8, piece c ^ (row / 2) % 8
   const int from = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
@@ -810,12 +822,12 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
     kpiece[i] = key_row * 128 + (((2 * i + hh) ^ ((key_row >> 1) & 7)) * 16);
     vpiece[i] = n * 128 + (((2 * i + hh) ^ ((n >> 1) & 7)) * 16);
   }
-  TileWalk walk;  // at the tile that loads last
+  const int64_t head_size = (int64_t)src.Tp * kHeadDim;
   TileAt ring[kRing - WK];  // the tiles in use and those on their way
   auto stage = [&](TileAt& x, int t) {
-    if (t == 0) walk.start(it, per_page, t0);
+    if (t == 0) walk.first();
     else walk.next();
-    x = walk.at(src, it, a.heads);
+    x = walk.at(src, it, a.heads, head_size);
     char* const to = lds + (t & (kRing - 1)) * 32 * kBlock;
     stage_tile<T>(src, x, klane, vlane, to, wave);
   };
@@ -824,6 +836,9 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
     ring[i] = TileAt{};
     if (i < n_own) stage(ring[i], i);
   }
+  // the queries' own wait, ahead of the loop's counted ones
+#pragma unroll
+  for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
   for (int t = 0; t < n_own; t += WK) {
     // This round's tiles have landed (a wave's loads land in order: what was issued after them may
     // still be under way), and everybody is done with the round before, whose buffers load next.
@@ -852,7 +867,7 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
       ahead_of_products();
       const bool partial = OWN && cur.key0 + cur.valid > it.open, masked = cur.valid < kTile || partial;
       if (masked) {
-        const int seen = lim - (int)cur.key0;
+        const int seen = lim - cur.key0;
         int most = (seen < cur.valid ? seen : cur.valid) - 8 * hh;
         asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
 #pragma unroll
@@ -921,7 +936,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
   if ((int)blockIdx.x < a.pre_grid) {
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
     constexpr int R = kind_rows(PK);
-    const int pair = at / a.pre_rb * 8 + xcd, rb = at % a.pre_rb;
+    // a padded batch's last row blocks may hold no tokens: they come last
+    const int per = a.pre_grid / 8 / a.pre_rb, pair = (a.new_lens ? at % per : at / a.pre_rb) * 8 + xcd;
+    const int rb = a.new_lens ? at / per : at % a.pre_rb;
     if (pair >= a.heads * a.pre_splits) return;
     it.h = pair % a.heads;
     it.split = it.part = pair / a.heads;
@@ -956,7 +973,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
     it.m1 = it.m0 + R < rows ? it.m0 + R : rows;
     it.list = a.pre_pages;
     it.n_list = (int)((a.pre_tokens + a.pre.T - 1) / a.pre.T);
-    it.n_keys = it.open = a.pre_tokens;
+    it.n_keys = it.open = (int)a.pre_tokens;
     it.first_lim = 0;
     it.causal = false;
     if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
@@ -989,10 +1006,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
   const int fresh = fresh_rows(a, b), l0 = rb * R / a.group, l1 = (it.m1 - 1 - b * per) / a.group;
   const int64_t length = a.lengths[b], cap = (int64_t)a.width * a.own.T;
   it.first_lim = length - fresh + 1;
-  it.n_keys = a.causal && it.first_lim + l1 < length ? it.first_lim + l1 : length;
-  if (it.n_keys > cap) it.n_keys = cap;
-  if (it.n_keys < 0 || l0 >= fresh || none) it.n_keys = 0;  // no row of the item is a new token
-  it.open = a.causal ? it.first_lim + l0 : it.n_keys;
+  int64_t keys = a.causal && it.first_lim + l1 < length ? it.first_lim + l1 : length;
+  if (keys > cap) keys = cap;
+  if (keys < 0 || l0 >= fresh || none) keys = 0;  // no row of the item is a new token
+  it.n_keys = (int)keys;
+  it.open = !a.causal ? it.n_keys : it.first_lim + l0 < 0 ? 0 : it.first_lim + l0 < keys ? (int)it.first_lim + l0 : it.n_keys;
   if constexpr (OK) tile_item<T, OK, true>(a, a.own, it, lds);
   else stream_item<T, true>(a, a.own, it, waves, reinterpret_cast<float*>(lds));
 }
