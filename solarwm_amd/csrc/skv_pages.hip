@@ -17,7 +17,8 @@ namespace {
 struct Pages {
   const int32_t* tables;
   int64_t table_st;
-  int width, n_pages, T, Tp, heads;
+  int64_t capacity;  // tokens of a table: width * T, below 2^31
+  int n_pages, T, Tp, heads;
   const int32_t* lengths;
   const int32_t* new_lens;
 
@@ -55,11 +56,9 @@ struct Place {
   int off;
 };
 __device__ inline Place place_of(const Pages& pg, int b, int64_t own) {
-  if (own < 0) return Place{-1, 0};
-  const int64_t p = own / pg.T;
-  if (p >= pg.width) return Place{-1, 0};
-  const int id = pg.tables[b * pg.table_st + p];
-  return Place{id < 0 || id >= pg.n_pages ? -1 : id, (int)(own - p * pg.T)};
+  if (own < 0 || own >= pg.capacity) return Place{-1, 0};
+  const int p = (int)own / pg.T, id = pg.tables[b * pg.table_st + p];
+  return Place{id < 0 || id >= pg.n_pages ? -1 : id, (int)own - p * pg.T};
 }
 
 // V of one token and head by one wave: a lane's two channels go to two rows of the page.
@@ -88,27 +87,27 @@ __device__ inline void v_tile(const AppendPagesArgs& a, int unit, uint32_t (&buf
   const int j = unit % a.v_tiles, bh = unit / a.v_tiles;
   const int h = bh % a.pg.heads, b = bh / a.pg.heads;
   const int n = a.pg.fresh(b, a.rows);
-  const int64_t o0 = a.pg.first(b, n), o1 = o0 + n, from = o0 > 0 ? o0 : 0;
-  if (from >= o1) return;
+  const int64_t first = a.pg.first(b, n), end = first + n < a.pg.capacity ? first + n : a.pg.capacity;
+  if (end <= (first > 0 ? first : 0)) return;
+  const int from = first > 0 ? (int)first : 0, to = (int)end;
   const int per_page = (a.pg.T + kTile - 1) / kTile;
-  const int64_t p0 = from / a.pg.T;
-  const int64_t tile = p0 * per_page + (from - p0 * a.pg.T) / kTile + j;
-  const int64_t p = tile / per_page;
-  const int t0 = (int)(tile - p * per_page) * kTile;  // first token of the tile in its page
-  const int64_t base = p * a.pg.T + t0;               // its own index
+  const int p0 = from / a.pg.T, tile = p0 * per_page + (from - p0 * a.pg.T) / kTile + j;
+  const int p = tile / per_page, t0 = (tile - p * per_page) * kTile;  // its page, its first token there
+  const int64_t base = (int64_t)p * a.pg.T + t0;                      // and that token's own index
+  if (base >= to) return;
   const int cap = a.pg.T - t0 < kTile ? a.pg.T - t0 : kTile;
-  const int lo = from > base ? (int)(from - base) : 0;
-  const int hi = o1 - base < cap ? (int)(o1 - base) : cap;
-  if (lo >= hi || p >= a.pg.width) return;
+  const int lo = from > base ? from - (int)base : 0, hi = to - (int)base < cap ? to - (int)base : cap;
+  if (lo >= hi) return;
   const int id = a.pg.tables[b * a.pg.table_st + p];
   if (id < 0 || id >= a.pg.n_pages) return;
+  const int64_t row0 = base - first;  // the call's row of the tile's first token
   const int tid = threadIdx.x, c = tid & 15;
   const T* v = static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh + 8 * c;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = (tid >> 4) + 16 * i;
     if (r >= lo && r < hi) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(v + (base + r - o0) * a.v_st);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(v + (row0 + r) * a.v_st);
 #pragma unroll
       for (int e = 0; e < 4; ++e) buf[r][4 * c + e] = w[e];
     }
@@ -1315,7 +1314,7 @@ extern "C" int skv_append_pages(const skv_append_pages_desc* d, skv_stream_t str
     }
   }
   AppendPagesArgs a{};
-  a.pg.tables = d->tables, a.pg.table_st = d->table_stride, a.pg.width = d->table_width;
+  a.pg.tables = d->tables, a.pg.table_st = d->table_stride, a.pg.capacity = (int64_t)d->table_width * d->page_tokens;
   a.pg.n_pages = d->n_pages, a.pg.T = d->page_tokens, a.pg.Tp = padded_tokens(d->page_tokens);
   a.pg.heads = d->kv_heads, a.pg.lengths = d->lengths, a.pg.new_lens = d->new_lens;
   a.q = d->q, a.q_sb = d->q_sb, a.q_st = d->q_st, a.q_sh = d->q_sh;

@@ -228,6 +228,8 @@ ATTENDS = [  # batch, rows, q heads, kv heads, prefix, page, lengths, new_lens
     (3, 33, 2, 1, 70, 64, [33, 200, 40], [33, 20, 0]),
     (1, 150, 1, 1, 500, 390, [700], None),        # 150 rows of a sequence
     (2, 70, 3, 1, 0, 1, [70, 90], None),          # pages of one token
+    (1, 1, 3, 1, 200, 64, [1500], None),          # a long sequence, split along its keys
+    (1, 40, 2, 1, 0, 64, [1300], None),
 ]
 
 
@@ -378,6 +380,28 @@ def test_many_splits_and_many_rows(gpu):
                 bar = HALF[BF] * (a + o.abs()) * (1 + 2.0**-6) + U * (320 * size + 64 + ks.shape[0] / 64) * a
                 err = (got[i, 0, h * hq // hkv:(h + 1) * hq // hkv].double() - o).abs() - bar
                 assert float(err.max()) <= 0, (b, i, h, float(err.max()))
+
+
+@pytest.mark.parametrize("b,rows,prefix", [(150, 1, 0), (150, 2, 100), (1100, 2, 64)])
+def test_many_short_sequences(gpu, b, rows, prefix):
+    """More sequences than CUs (several share a workgroup) and more than the 1024 whose padding rows
+    close up, against the same call for one sequence at a time on the first, the last and some between."""
+    page, hkv, hq = 16, 2, 4
+    kpool, vpool = (t.to(gpu) for t in _pools(2 * b + 7, hkv, page, BF, "cpu", 171))
+    tables = torch.randperm(2 * b, generator=_gen(173)).int().reshape(b, 2).to(gpu)
+    ids = torch.arange(2 * b, 2 * b + 7, dtype=torch.int32, device=gpu)
+    new = [rows if i % 3 else i % 2 for i in range(b)]
+    lengths = [min(2 * page, new[i] + (11 * i) % 31) for i in range(b)]
+    q = torch.randn(b, rows, hq, D, generator=_gen(174)).to(BF).to(gpu)
+    lens, news = _i32(lengths, gpu), _i32(new, gpu)
+    got = attend_shared(q, kpool, vpool, tables, lens, page_tokens=page, prefix_pages=ids, prefix_tokens=prefix,
+                        new_lens=news)
+    for i in [0, 1, 2, b // 2, b // 2 + 1, b - 2, b - 1]:
+        want, bar = _attention(q[i:i + 1].cpu(), (kpool.cpu(), vpool.cpu(), page, tables[i:i + 1].cpu()),
+                               lengths[i:i + 1], new[i:i + 1], True,
+                               (kpool.cpu(), vpool.cpu(), page, ids.tolist(), prefix) if prefix else None)
+        _check(got[i:i + 1], want, bar, i)
+        assert not got[i, new[i]:].any()
 
 
 def test_pools_past_32_bit_offsets(gpu):
