@@ -256,6 +256,7 @@ struct SharedArgs {
   int pre_rb, pre_splits, pre_grid;  // row blocks, key splits and workgroups of the prefix
   int own_rb, own_splits, own_items, own_waves;  // row blocks of a sequence, key splits; waves of an item
   int direct;    // one part only: workgroups write out themselves
+  int both;      // one sequence, few rows: prefix and own keys in one work item
   float* part_o;   // [part][heads][M][128]
   float2* part_ml; // [part][heads][M]
 };
@@ -442,36 +443,45 @@ __device__ inline float row_out(const SharedArgs& a, const Item& it, int m, floa
 // ---- at most 16 rows: a wave streams its own keys, 32 a step, on 16x16x32 MFMAs ----------------
 // Row i of S tile t is key (i / 4) * 8 + 4 t + i % 4 of the step; lane (n, g) holds row n's keys
 // 8 g .. 8 g + 7.
-// `waves` of the workgroup (1, 2, 4 or 8, the same for all its items) work on one item, this one of them
-// being number wk.  All waves of the workgroup come here: those without an item with m0 == m1.
-template <typename T, bool OWN>
-__device__ inline void stream_item(const SharedArgs& a, const Source& src, const Item& it, int waves, float* lds) {
-  typedef typename Mma<T>::v8 v8;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wk = wave & (waves - 1), n = lane & 15, g = lane >> 4;
-  const int per_page = (src.T + kStep - 1) / kStep;
-  const int n_steps = steps_of(src, it.n_keys, kStep, per_page);
-  const int share = it.n_split * waves, mine = it.split * waves + wk;
-  const int s0 = share_of(n_steps, mine, share), s1 = share_of(n_steps, mine + 1, share);
-  PageWalk pages;
-  int page = s0 / per_page, in_page = s0 - page * per_page;
-  if (s0 < s1) pages.start(it.list, it.n_list, page);  // loads while the rows are looked up
-  const int m = it.m0 + n;
-  int b, l, gh;
-  row_of(a, m < it.m1 ? m : it.m0, b, l, gh);
-  const int lim = OWN && it.causal ? (int)(it.first_lim + l > 0 ? it.first_lim + l : 0) : it.n_keys;
-  v8 q[4];
-  {
-    const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
-                 (int64_t)(it.h * a.group + gh) * a.q_sh + g * 8;
-#pragma unroll
-    for (int st = 0; st < 4; ++st) q[st] = *reinterpret_cast<const v8*>(p + st * 32);
-  }
+template <typename T>
+struct StreamState {
+  typename Mma<T>::v8 q[4];
   f32x4 o[8];
+  float mx, sum;
+  int m, lim;  // the lane's row (m1 and beyond: none), and how many own keys it sees
+};
+
+template <typename T>
+__device__ inline void stream_begin(StreamState<T>& w, const SharedArgs& a, const Item& it) {
+  const int lane = threadIdx.x & 63;
+  w.m = it.m0 + (lane & 15);
+  int b, l, gh;
+  row_of(a, w.m < it.m1 ? w.m : it.m0, b, l, gh);
+  w.lim = it.causal ? (int)(it.first_lim + l > 0 ? it.first_lim + l : 0) : it.n_keys;
+  const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
+               (int64_t)(it.h * a.group + gh) * a.q_sh + (lane >> 4) * 8;
 #pragma unroll
-  for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float mx = -INFINITY, sum = 0.0f;
+  for (int st = 0; st < 4; ++st) w.q[st] = *reinterpret_cast<const typename Mma<T>::v8*>(p + st * 32);
+#pragma unroll
+  for (int d = 0; d < 8; ++d) w.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  w.mx = -INFINITY;
+  w.sum = 0.0f;
+}
+
+// Steps [s0, s1) of an item's keys.
+template <typename T, bool OWN>
+__device__ inline void stream_steps(StreamState<T>& w, const SharedArgs& a, const Source& src, const Item& it,
+                                    int per_page, int s0, int s1) {
+  typedef typename Mma<T>::v8 v8;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  v8 (&q)[4] = w.q;
+  f32x4 (&o)[8] = w.o;
+  float mx = w.mx, sum = w.sum;
+  const int lim = OWN ? w.lim : it.n_keys;
   if (s0 < s1) {
+    PageWalk pages;
+    int page = s0 / per_page, in_page = s0 - page * per_page;
+    pages.start(it.list, it.n_list, page);
     const int k_off = ((n >> 2) * 8 + (n & 3)) * kHeadDim + g * 8, v_off = n * src.Tp + g * 8;
     const T* kp = static_cast<const T*>(src.k_pool);
     const T* vp = static_cast<const T*>(src.v_pool);
@@ -575,8 +585,18 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
       for (int d = 0; d < 8; ++d) o[d] = Mma<T>::mul(vf[d], p, o[d]);
     }
   }
-  sum = over_groups_sum(sum, 16);
-  // the waves' shares join in halves through LDS: 32 outputs, m and l of a lane
+  w.mx = mx;
+  w.sum = sum;
+}
+
+// The `waves` of an item, this one of them being number wk, join in halves through LDS (32 outputs, m and
+// l of a lane); the first of them writes the item's part.
+template <typename T>
+__device__ inline void stream_end(StreamState<T>& w, const SharedArgs& a, const Item& it, int wave, int waves,
+                                  float* lds) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, wk = wave & (waves - 1);
+  f32x4 (&o)[8] = w.o;
+  float mx = w.mx, sum = over_groups_sum(w.sum, 16);
   for (int half = waves >> 1; half > 0; half >>= 1) {
     float* at = lds + (wave / waves * (waves >> 1) + (wk & (half - 1))) * 34 * 64 + lane;
     if (wk >= half && wk < 2 * half) {
@@ -597,11 +617,39 @@ __device__ inline void stream_item(const SharedArgs& a, const Source& src, const
     }
     __syncthreads();
   }
-  if (wk > 0 || m >= it.m1) return;
+  if (wk > 0 || w.m >= it.m1) return;
   T* dst = nullptr;
-  const float inv = row_out<T>(a, it, m, mx, sum, g == 0, &dst);
+  const float inv = row_out<T>(a, it, w.m, mx, sum, g == 0, &dst);
 #pragma unroll
-  for (int d = 0; d < 8; ++d) put4<T>(a, it, m, 16 * d + 4 * g, o[d], inv, dst);
+  for (int d = 0; d < 8; ++d) put4<T>(a, it, w.m, 16 * d + 4 * g, o[d], inv, dst);
+}
+
+// `waves` of the workgroup (1, 2, 4 or 8, the same for all its items) work on one item.  All waves of the
+// workgroup come here: those without an item with m0 == m1.
+template <typename T, bool OWN>
+__device__ inline void stream_item(const SharedArgs& a, const Source& src, const Item& it, int waves, float* lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per_page = (src.T + kStep - 1) / kStep, n_steps = steps_of(src, it.n_keys, kStep, per_page);
+  const int share = it.n_split * waves, mine = it.split * waves + (wave & (waves - 1));
+  StreamState<T> w;
+  stream_begin(w, a, it);
+  stream_steps<T, OWN>(w, a, src, it, per_page, share_of(n_steps, mine, share), share_of(n_steps, mine + 1, share));
+  stream_end(w, a, it, wave, waves, lds);
+}
+
+// The only sequence of a call with few rows: the prefix's keys and then its own, one after the other.
+template <typename T>
+__device__ inline void stream_both(const SharedArgs& a, const Item& pre, const Item& own, float* lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pp = (a.pre.T + kStep - 1) / kStep, po = (a.own.T + kStep - 1) / kStep;
+  const int n_pre = steps_of(a.pre, pre.n_keys, kStep, pp), n = n_pre + steps_of(a.own, own.n_keys, kStep, po);
+  const int share = own.n_split * kWaves, mine = own.split * kWaves + wave;
+  const int s0 = share_of(n, mine, share), s1 = share_of(n, mine + 1, share);
+  StreamState<T> w;
+  stream_begin(w, a, own);
+  stream_steps<T, false>(w, a, a.pre, pre, pp, s0, s1 < n_pre ? s1 : n_pre);
+  stream_steps<T, true>(w, a, a.own, own, po, s0 < n_pre ? 0 : s0 - n_pre, s1 - n_pre);
+  stream_end(w, a, own, wave, kWaves, lds);
 }
 
 // ---- more rows: waves of 32 rows share tiles of 64 keys in LDS, on 32x32x16 MFMAs ---------------
@@ -924,6 +972,32 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
 }
 
 
+__device__ inline void prefix_keys(const SharedArgs& a, Item& it) {
+  it.list = a.pre_pages;
+  it.n_list = (int)((a.pre_tokens + a.pre.T - 1) / a.pre.T);
+  it.n_keys = it.open = (int)a.pre_tokens;
+  it.first_lim = 0;
+  it.causal = false;
+}
+
+// The keys of sequence b that rows [m0, m1) see; `none`: there is no item.
+__device__ inline void own_keys(const SharedArgs& a, Item& it, int b, bool none) {
+  const int per = a.rows * a.group;
+  it.tokens = nullptr;
+  it.list = a.tables + b * a.table_st;
+  it.n_list = a.width;
+  it.causal = a.causal;
+  // row l of a causal sequence sees lengths - fresh + l + 1 keys; keys past the table do not exist
+  const int fresh = fresh_rows(a, b), l0 = (it.m0 - b * per) / a.group, l1 = (it.m1 - 1 - b * per) / a.group;
+  const int64_t length = a.lengths[b], cap = (int64_t)a.width * a.own.T;
+  it.first_lim = length - fresh + 1;
+  int64_t keys = a.causal && it.first_lim + l1 < length ? it.first_lim + l1 : length;
+  if (keys > cap) keys = cap;
+  if (keys < 0 || l0 >= fresh || none) keys = 0;  // no row of the item is a new token
+  it.n_keys = (int)keys;
+  it.open = !a.causal ? it.n_keys : it.first_lim + l0 < 0 ? 0 : it.first_lim + l0 < keys ? (int)it.first_lim + l0 : it.n_keys;
+}
+
 // The prefix's work items first, dealt so that the row blocks of one (key head, split) run one after
 // another on one XCD and share its L2; then every sequence's own pages.  PK, OK: how the prefix and the
 // own pages go (0: streaming, else tiles a round).
@@ -932,6 +1006,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
   __shared__ __attribute__((aligned(16))) char lds[PK || OK ? kTileLds : kWaves / 2 * 34 * 64 * 4];
   __shared__ int tokens[PK ? kCompact + 1 : 1];
   Item it;
+  if constexpr (PK == 0 && OK == 0) {
+    if (a.both) {
+      Item pre;
+      it.h = pre.h = blockIdx.x % a.heads;
+      it.split = it.part = blockIdx.x / a.heads;
+      it.n_split = a.pre_splits;
+      it.m0 = 0;
+      it.m1 = a.M;
+      prefix_keys(a, pre);
+      own_keys(a, it, 0, false);
+      stream_both<T>(a, pre, it, reinterpret_cast<float*>(lds));
+      return;
+    }
+  }
   if ((int)blockIdx.x < a.pre_grid) {
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
     constexpr int R = kind_rows(PK);
@@ -970,11 +1058,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
     }
     it.m0 = rb * R;
     it.m1 = it.m0 + R < rows ? it.m0 + R : rows;
-    it.list = a.pre_pages;
-    it.n_list = (int)((a.pre_tokens + a.pre.T - 1) / a.pre.T);
-    it.n_keys = it.open = (int)a.pre_tokens;
-    it.first_lim = 0;
-    it.causal = false;
+    prefix_keys(a, it);
     if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
     else stream_item<T, false>(a, a.pre, it, kWaves, reinterpret_cast<float*>(lds));
     return;
@@ -997,19 +1081,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
   it.m0 = b * per + rb * R;
   it.m1 = it.m0 + R < (b + 1) * per ? it.m0 + R : (b + 1) * per;
   if (none) it.m1 = it.m0;
-  it.tokens = nullptr;
-  it.list = a.tables + b * a.table_st;
-  it.n_list = a.width;
-  it.causal = a.causal;
-  // row l of a causal sequence sees lengths - fresh + l + 1 keys; keys past the table do not exist
-  const int fresh = fresh_rows(a, b), l0 = rb * R / a.group, l1 = (it.m1 - 1 - b * per) / a.group;
-  const int64_t length = a.lengths[b], cap = (int64_t)a.width * a.own.T;
-  it.first_lim = length - fresh + 1;
-  int64_t keys = a.causal && it.first_lim + l1 < length ? it.first_lim + l1 : length;
-  if (keys > cap) keys = cap;
-  if (keys < 0 || l0 >= fresh || none) keys = 0;  // no row of the item is a new token
-  it.n_keys = (int)keys;
-  it.open = !a.causal ? it.n_keys : it.first_lim + l0 < 0 ? 0 : it.first_lim + l0 < keys ? (int)it.first_lim + l0 : it.n_keys;
+  own_keys(a, it, b, none);
   if constexpr (OK) tile_item<T, OK, true>(a, a.own, it, lds);
   else stream_item<T, true>(a, a.own, it, waves, reinterpret_cast<float*>(lds));
 }
@@ -1118,6 +1190,7 @@ int common_errors(const char* fn, int dtype, int head_dim, int batch, int rows, 
 // The launch of an attention: whether each kind of work item goes by tiles, and the splits.
 struct SharedPlan {
   int pre_kind, own_kind;
+  bool both;  // one sequence with few rows: the prefix's keys and its own make one list
   int pre_rb, pre_splits, pre_grid, own_rb, own_splits, own_items, own_waves, own_grid, parts;
   int64_t bytes;
 };
@@ -1130,7 +1203,7 @@ struct SharedPlan {
 // partial results and the merge.
 void choose_splits(const skv_attend_shared_desc* d, int64_t M, int64_t cu, int64_t pre_items, int64_t pre_tiles,
                    int64_t own_items, int64_t own_tiles, SharedPlan* p) {
-  constexpr double kFixed = 7.0, kBytes = 4.6e6, kMerge = 5.0, kTileBytes = 32768.0;
+  constexpr double kFixed = 7.0, kBytes = 4.6e6, kMerge = 7.0, kTileBytes = 32768.0;
   auto tile_cost = [](int kind, double busy) {
     const double over = (busy < 1.0 ? busy : 1.0) - 0.65;
     return kind == 0 ? 0.86 : kind == 2 ? 1.15 : 1.7 + (over > 0 ? 1.4 * over : 0.0);
@@ -1147,11 +1220,12 @@ void choose_splits(const skv_attend_shared_desc* d, int64_t M, int64_t cu, int64
   p->pre_splits = pre_tiles > 0, p->own_splits = own_tiles > 0, p->own_waves = waves;
   for (int os = 1; os <= (waves == kWaves && own_tiles > 1 ? 32 : 1); os *= 2) {
     const int64_t n_own = own_tiles ? (own_items * os * waves + kWaves - 1) / kWaves : 0;
-    // the prefix's workgroups fill what the own ones leave of a round or two, or a part of a round
-    for (int f = 0; f < (pre_tiles ? 6 : 1); ++f) {
+    // the prefix's workgroups fill what the own ones leave of a round or two, or a part of a round; or one
+    // part each
+    for (int f = 0; f < (pre_tiles ? 7 : 1); ++f) {
       int64_t ps = 0;
       if (pre_tiles) {
-        const int64_t room = f == 0 ? cu - n_own : f == 1 ? 2 * cu - n_own : cu * (f - 1) / 4;
+        const int64_t room = f == 0 ? cu - n_own : f == 1 ? 2 * cu - n_own : f < 6 ? cu * (f - 1) / 4 : 0;
         ps = room / pre_items;
         ps = ps < 1 ? 1 : ps > pre_tiles ? pre_tiles : ps > 256 ? 256 : ps;
       }
@@ -1205,7 +1279,9 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
   const int64_t own_items = (int64_t)p->own_rb * d->kv_heads * d->batch;
   // of a padded batch's row blocks about half hold tokens
   const int64_t busy_rb = d->new_lens && p->pre_kind ? (M / 2 + pre_rows) / pre_rows : p->pre_rb;
-  choose_splits(d, M, cu, busy_rb < p->pre_rb ? busy_rb * d->kv_heads : pre_items, pre_tiles, own_items, own_tiles, p);
+  p->both = pre && own && d->batch == 1 && p->pre_kind == 0;
+  if (p->both) choose_splits(d, M, cu, pre_items, pre_tiles + own_tiles, 0, 0, p);
+  else choose_splits(d, M, cu, busy_rb < p->pre_rb ? busy_rb * d->kv_heads : pre_items, pre_tiles, own_items, own_tiles, p);
   p->parts = p->pre_splits + p->own_splits;
   const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits, each = p->own_kind ? 1 : kWaves / p->own_waves;
   const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, all_own = own_items * p->own_splits;
@@ -1213,9 +1289,9 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
     set_error("%s: too many work items", fn);
     return SKV_E_ARG;
   }
-  p->pre_grid = (int)pre_grid;
+  p->pre_grid = p->both ? (int)pairs : (int)pre_grid;
   p->own_items = (int)all_own;
-  p->own_grid = (int)((all_own + each - 1) / each);
+  p->own_grid = p->both ? 0 : (int)((all_own + each - 1) / each);
   p->bytes = p->parts > 1 ? (int64_t)p->parts * d->kv_heads * M * (kHeadDim * 4 + 8) : 0;
   return SKV_OK;
 }
@@ -1408,7 +1484,7 @@ extern "C" int skv_attend_shared(const skv_attend_shared_desc* d, skv_stream_t s
   a.pre_rb = p.pre_rb, a.pre_splits = p.pre_splits, a.pre_grid = p.pre_grid;
   a.own_rb = p.own_rb, a.own_splits = p.own_splits;
   a.own_items = p.own_items, a.own_waves = p.own_waves;
-  a.direct = p.parts == 1;
+  a.direct = p.parts == 1, a.both = p.both;
   a.part_o = static_cast<float*>(d->workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)p.parts * a.heads * a.M * kHeadDim);
   hipStream_t s = static_cast<hipStream_t>(stream);
