@@ -524,8 +524,9 @@ int skv_qk_norm_rope_grad_workspace(const skv_qk_norm_rope_desc* desc, int64_t* 
  * (as skv_qk_norm_rope), and the queries with them into q_out (q_heads = 0 leaves them out).  The
  * table row of a token's rotation is position0 + positions[b][t], or without `positions`
  * position0 + its own index (position0 = tokens of the shared prefix).  Rows that are no new tokens
- * and tokens without a page write no K and V; q_out rows that are no new tokens are zero.  A page is
- * written by one sequence of a call (two tokens of one place leave either's values).
+ * and tokens without a page write no K and V; q_out rows that are no new tokens are zero; q_out may be
+ * q itself, and must not otherwise overlap an input.  A page is written by one sequence of a call (two
+ * tokens of one place leave either's values).
  * (Replaces the scatter of normalised, rotated K and of V into a pooled cache,
  * deploy/solar_wm/shared/vae/streamrender_tp.py:21-60.)
  */
@@ -572,8 +573,9 @@ int skv_append_pages(const skv_append_pages_desc* desc, skv_stream_t stream);
  * with q and out [batch][rows][q_heads][128] views (16-byte aligned, strides non-negative multiples
  * of 8) and q_heads a multiple of kv_heads.  `causal`: row t of a sequence sees its first
  * lengths[b] - new_lens[b] + t + 1 own tokens; otherwise all lengths[b].  Keys of pages that are not
- * there are not seen; a row that sees no key, and rows that are no new tokens, are zero.  What pages
- * hold behind their tokens does not matter, infinities and NaN included.  bf16 / f16 matrix-core
+ * there are not seen; a row that sees no key, and rows that are no new tokens, are zero; out may be q
+ * itself, and must not otherwise overlap an input.  What pages hold behind their tokens does not
+ * matter, infinities and NaN included.  bf16 / f16 matrix-core
  * products with fp32 accumulation and an fp32 online softmax; every part of the keys leaves fp32
  * partial results in the workspace that skv_attend_shared_workspace reports for the same descriptor
  * (16-byte aligned, used by the call only), joined in a fixed order.

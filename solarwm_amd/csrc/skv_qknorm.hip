@@ -244,7 +244,7 @@ QkSide side(const skv_norm_side& s) {
   o.g = s.grad, o.gb = s.grad_sb, o.gt = s.grad_st, o.gh = s.grad_sh;
   o.out = s.out, o.ob = s.out_sb, o.ot = s.out_st, o.oh = s.out_sh;
   o.w = s.norm ? s.weight : nullptr, o.w_dtype = s.weight_dtype, o.norm = s.norm != 0;
-  o.heads = s.heads, o.blocks = (s.heads + kHeadBlock - 1) / kHeadBlock, o.eps = s.eps;
+  o.heads = s.heads, o.blocks = head_blocks(s.heads), o.eps = s.eps;
   o.dw = s.grad_weight, o.dw_dtype = s.grad_weight_dtype;
   return o;
 }
@@ -286,7 +286,7 @@ int fill(const char* fn, const skv_qk_norm_rope_desc* d, bool grad, QkArgs* a) {
   a->q = side(d->q);
   if (d->k.heads) a->k = side(d->k);
   const int64_t tokens = (int64_t)d->batch * d->rows;
-  if (tokens * (a->q.blocks + a->k.blocks) + 16 * 4096 >= ((int64_t)1 << 31)) {
+  if (tokens >= ((int64_t)1 << 31) || (tokens * (a->q.blocks + (int64_t)a->k.blocks) + 15) / 16 * 256 >= kMaxThreads) {
     set_error("%s: too many rows (batch=%d rows=%d)", fn, d->batch, d->rows);
     return SKV_E_ARG;
   }

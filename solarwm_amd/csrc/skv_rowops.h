@@ -8,6 +8,9 @@ namespace skv {
 
 constexpr int kRowLanes = 16;  // lanes per 128-channel head row
 constexpr int kHeadBlock = 4;  // heads of one token that a group works on with one table row
+inline int head_blocks(int heads) { return heads / kHeadBlock + (heads % kHeadBlock > 0); }
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;  // a launch has fewer
+
 
 // 8 channels as raw words: 4 of a 16-bit type, 8 of float.
 template <typename T>

@@ -65,6 +65,13 @@ def _int32_vector(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
     return t
 
 
+def _check_out(out: torch.Tensor, q: torch.Tensor) -> None:
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must match q's shape and dtype")
+    if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+        raise ValueError("out must not be expanded: its rows would lie on one another")
+
+
 def _set_pages(d, kpool, vpool, n_pages, page_tokens, tables, lengths, new_lens, batch) -> None:
     """The fields that both descriptors share."""
     if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != batch:
@@ -110,7 +117,8 @@ def append_pages(
     where given, so ``position0`` is the length of a shared prefix.
 
     ``q`` [B, L, Hq, 128] goes through ``norm_q`` and the same rotation; the result (or ``out``, which
-    may be ``q`` itself) is returned, with zeros in rows that are no new tokens.  Rows that are no new
+    may be ``q`` itself and must not otherwise share memory with an input) is returned, with zeros in
+    rows that are no new tokens.  No gradient is recorded.  Rows that are no new
     tokens and tokens whose page is not there leave the pools as they were.  Each page takes tokens of
     one sequence only; where two tokens of a call share a place, either's values may stay."""
     check_heads("k", k, _HALVES)
@@ -137,8 +145,8 @@ def append_pages(
             raise ValueError(f"q must share k's dtype, batch and length, got {q.dtype} {tuple(q.shape)}")
         if out is None:
             out = empty_as(q)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must match q's shape and dtype")
+        else:
+            _check_out(out, q)
         d.q, d.q_out, d.q_heads = q.data_ptr(), out.data_ptr(), q.shape[2]
         d.q_sb, d.q_st, d.q_sh = strides("q", q)
         d.out_sb, d.out_st, d.out_sh = strides("out", out)
@@ -193,7 +201,8 @@ def attend_shared(
     pools or of ``prefix_pools = (kpool, vpool, page_tokens)``; every row sees all of it, and its keys
     are read once for the whole batch.  Of its own tokens row t of a sequence sees the first
     ``lengths[b] - new_lens[b] + t + 1`` (``causal``) or all ``lengths[b]``.  Rows that are no new
-    tokens, and rows that see no key at all, come back as zeros."""
+    tokens, and rows that see no key at all, come back as zeros.  ``out`` may be ``q`` itself, and must
+    not otherwise share memory with an input.  No gradient is recorded."""
     check_heads("q", q, _HALVES)
     b, l, hq, _ = q.shape
     n_pages, h = _check_pools("", kpool, vpool, page_tokens, q.dtype)
@@ -225,8 +234,8 @@ def attend_shared(
         prefix_pages = None
     if out is None:
         out = empty_as(q)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must match q's shape and dtype")
+    else:
+        _check_out(out, q)
     d.q, d.out = q.data_ptr(), out.data_ptr()
     d.q_sb, d.q_st, d.q_sh = strides("q", q)
     d.out_sb, d.out_st, d.out_sh = strides("out", out)

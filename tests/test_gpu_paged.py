@@ -353,6 +353,30 @@ def test_strides_scale_and_other_pools(gpu):
     assert got.data_ptr() == out.data_ptr() and (out[:, :, 1::2] == 7.0).all()
 
 
+@pytest.mark.parametrize("b,n,hq,prefix", [(1, 1, 4, 100), (1, 3, 4, 5000), (3, 5, 6, 900), (2, 70, 2, 0), (40, 1, 8, 700)])
+def test_out_is_q(gpu, b, n, hq, prefix):
+    """Both operators write over their queries: the bits of a call with an output of its own."""
+    hkv, page = 2, 64
+    n_pre = -(-prefix // page)
+    kpool, vpool = (t.to(gpu) for t in _pools(n_pre + 3 * b, hkv, page, BF, "cpu", 91))
+    order = torch.randperm(n_pre + 3 * b, generator=_gen(92)).int().to(gpu)
+    ids, tables = order[:n_pre].contiguous(), order[n_pre:].reshape(b, 3)
+    lengths = torch.randint(n, 3 * page + 1, (b,), generator=_gen(93), dtype=torch.int32).to(gpu)
+    q = torch.randn(b, n, hq, D, generator=_gen(94)).to(BF).to(gpu)
+    k, v = (torch.randn(b, n, hkv, D, generator=_gen(95 + i)).to(BF).to(gpu) for i in range(2))
+    angle = torch.rand(8192, 64, generator=_gen(97)).to(gpu)
+    rope = dict(cos=angle.cos(), sin=angle.sin(), position0=prefix, norm_q=(None, 1e-6), norm_k=(None, 1e-6))
+
+    def step(q, out):
+        q = append_pages(k, v, kpool, vpool, tables, lengths, page_tokens=page, q=q, out=out, **rope)
+        return attend_shared(q, kpool, vpool, tables, lengths, page_tokens=page, prefix_pages=ids,
+                             prefix_tokens=prefix, out=out)
+
+    want = step(q, None)
+    got = step(q, q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+
+
 def test_many_splits_and_many_rows(gpu):
     """A long prefix split over the chip for few rows, and for many row blocks, against float64 on the
     GPU (float64 products of the same pools)."""

@@ -57,6 +57,7 @@ COMMON = [
     ("norm_k weight", dict(norm_k=(torch.zeros(2 * D), 1e-6))),
     ("norm_q / out without q", dict(q=None, norm_q=(None, 1e-6))),
     ("out must match", dict(out=_x(2, 3, 2, D))),
+    ("must not be expanded", dict(out=_x(1, 3, 4, D).expand(2, 3, 4, D))),
     ("contiguous in its last", dict(v=_x(2, 3, D, 2).transpose(2, 3))),
 ])
 def test_append_refusals(text, kw):
@@ -80,6 +81,7 @@ def test_append_refusals(text, kw):
     ("prefix pool shapes", dict(prefix_tokens=1, prefix_pages=torch.zeros(1, dtype=torch.int32),
                                 prefix_pools=(_x(1, 1, 2, 64, D), _x(1, 1, 2, D, 64), 65))),
     ("out must match", dict(out=_x(2, 3, 4, D, dtype=torch.float16))),
+    ("must not be expanded", dict(out=_x(2, 3, 1, D).expand(2, 3, 4, D))),
 ])
 def test_attend_refusals(text, kw):
     a = _args(**kw)
@@ -164,3 +166,36 @@ def test_attend_descriptor_errors_do_not_launch(status, text, kw):
     assert lib.skv_attend_shared(ctypes.byref(d), None) == status
     assert text in lib.skv_last_error()
     assert lib.skv_attend_shared(None, None) == _lib.SKV_E_ARG
+
+
+PREFIX = dict(prefix_tokens=64, prefix_k_pool=0x1000, prefix_v_pool=0x1000, prefix_n_pages=1,
+              prefix_page_tokens=64, prefix_pages=0x1000)
+
+
+@pytest.mark.parametrize("kw", [dict(batch=0), dict(rows=0), dict(batch=1, rows=0), dict(batch=0, **PREFIX),
+                                dict(rows=0, **PREFIX), dict(batch=1, rows=0, **PREFIX)])
+def test_nothing_to_do(kw):
+    """No sequences or no rows: nothing is launched, with and without a prefix."""
+    lib, size = _lib.load(), ctypes.c_int64(-1)
+    d = _desc(_lib.AttendSharedDesc, **kw)
+    assert lib.skv_attend_shared_workspace(ctypes.byref(d), ctypes.byref(size)) == 0 and size.value == 0
+    assert lib.skv_attend_shared(ctypes.byref(d), None) == 0
+    d = _desc(_lib.AppendPagesDesc, **{k: v for k, v in kw.items() if not k.startswith("prefix")})
+    assert lib.skv_append_pages(ctypes.byref(d), None) == 0
+
+
+MOST = (1 << 31) - 1
+
+
+@pytest.mark.parametrize("kw", [
+    dict(batch=MOST, rows=MOST), dict(batch=MOST, rows=MOST, q_heads=MOST, kv_heads=MOST),
+    dict(batch=1, rows=MOST, q_heads=MOST, kv_heads=MOST), dict(batch=1 << 28, rows=1, q_heads=2, kv_heads=1),
+    dict(batch=MOST, rows=1, q_heads=MOST, kv_heads=1, page_tokens=1),
+])
+def test_sizes_past_a_launch(kw):
+    """Sizes that no launch takes are refused, whatever their products wrap to."""
+    lib = _lib.load()
+    for kind, entry in ((_lib.AttendSharedDesc, "skv_attend_shared"), (_lib.AppendPagesDesc, "skv_append_pages")):
+        d = _desc(kind, **kw)
+        assert getattr(lib, entry)(ctypes.byref(d), None) == _lib.SKV_E_ARG
+        assert b"too many" in lib.skv_last_error()

@@ -109,3 +109,14 @@ def test_gradient_errors_do_not_launch():
     assert lib.skv_qk_norm_rope_grad(ctypes.byref(d), None) == _lib.SKV_E_ARG
     assert b"grad_weight" in lib.skv_last_error()
     assert lib.skv_qk_norm_rope(None, None) == _lib.SKV_E_ARG
+
+
+@pytest.mark.parametrize("entry", ["skv_qk_norm_rope", "skv_qk_norm_rope_grad"])
+@pytest.mark.parametrize("kw", [dict(batch=(1 << 31) - 1, rows=(1 << 31) - 1), dict(batch=1, rows=1 << 28),
+                                dict(batch=1, rows=1 << 30, q_side_heads=(1 << 31) - 1, q_side_x_sh=0,
+                                     q_side_out_sh=0)])
+def test_sizes_past_a_launch(entry, kw):
+    lib = _lib.load()
+    d = _desc(q_side_x_st=0, q_side_out_st=0, k_side_x_st=0, k_side_out_st=0, **kw)
+    assert getattr(lib, entry)(ctypes.byref(d), None) == _lib.SKV_E_ARG
+    assert b"too many rows" in lib.skv_last_error()
