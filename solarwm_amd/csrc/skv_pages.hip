@@ -694,19 +694,31 @@ struct TileWalk {
 
 // A wave's share of a tile: 8 keys of K and twice 8 channels of V^T.  `lane` and `dst` are its own.
 template <typename T>
-__device__ inline void stage_tile(const Source& src, const TileAt& x, int klane, int vlane, lds_char* dst, int wave) {
+__device__ inline void stage_k(const Source& src, const TileAt& x, int klane, lds_char* dst, int wave) {
   const T* kt = static_cast<const T*>(src.k_pool) + x.base + x.tok0 * kHeadDim;
-  const T* vt = static_cast<const T*>(src.v_pool) + x.base + x.tok0;
   const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kt, (short)0, 0x7fffffff, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vt, (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(dst + (8 * i + wave) * kBlock), 16, klane,
                                              (8 * wave * kHeadDim + 64 * i) * 2, 0, 0);
+}
+template <typename T>
+__device__ inline void stage_v(const Source& src, const TileAt& x, int vlane, lds_char* dst, int wave) {
+  const T* vt = static_cast<const T*>(src.v_pool) + x.base + x.tok0;
+  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vt, (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (16 + 8 * i + wave) * kBlock), 16, vlane,
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (8 * i + wave) * kBlock), 16, vlane,
                                              8 * (wave + 8 * i) * src.Tp * 2, 0, 0);
+}
+
+// Where a load into `at` of LDS goes, as a number that hipcc cannot trace to the array: where it can, it
+// waits for every load under way ahead of a round's first read (7 to 14% of a tile's time); the loops
+// below count their waits.
+__device__ inline lds_char* load_target(char* at) {
+  uint32_t to = (uint32_t)(uintptr_t)(lds_char*)at;
+  asm volatile("" : "+s"(to));
+  return (lds_char*)(uintptr_t)to;
 }
 
 // 16 products with their LDS operands read four ahead.
@@ -743,8 +755,9 @@ __device__ inline float probs(const f32x16 (&sc)[2], float c, float mx, typename
 }
 
 template <typename T>
-__device__ inline void settle(TileState<T>& w, const f32x16 (&sc)[2], float c, float sum, typename Mma<T>::v8 (&p)[4]) {
-  if (__any(!(sum <= 256.0f) || w.mx == -INFINITY)) {
+__device__ inline void settle(TileState<T>& w, const f32x16 (&sc)[2], float c, float sum, typename Mma<T>::v8 (&p)[4],
+                              bool odd) {
+  if (__any(odd)) {
     float top = sc[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) top = fmaxf(top, sc[i >> 4][i & 15]);
@@ -813,6 +826,66 @@ __device__ inline void masked_pv(TileState<T>& w, const TileAt& x, bool partial,
   }
 }
 
+// Queries and an empty state of row m, and where a lane's loads and operand reads lie.
+template <typename T>
+__device__ inline void tile_begin(TileState<T>& w, const SharedArgs& a, const Item& it, int m, int hh) {
+  int b, l, gh;
+  row_of(a, m, b, l, gh);
+  const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
+               (int64_t)(it.h * a.group + gh) * a.q_sh + hh * 8;
+#pragma unroll
+  for (int st = 0; st < 8; ++st) w.q[st] = *reinterpret_cast<const typename Mma<T>::v8*>(p + st * 16);
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
+  w.mx = -INFINITY;
+  w.sum = 0.0f;
+}
+__device__ inline void tile_lanes(const Source& src, int wave, int lane, int& klane, int& vlane, int (&kpiece)[4],
+                                  int (&vpiece)[4]) {
+  const int n = lane & 31, hh = lane >> 5, key_row = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+  // loads: lane (r, c) of a wave takes row r of its 8, piece c ^ (row / 2) % 8
+  const int from = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
+  klane = ((lane >> 3) * kHeadDim + from * 8) * 2;
+  vlane = ((lane >> 3) * src.Tp + from * 8) * 2;
+  // operand reads: where pieces 2 i + hh of the lane's K row and V^T row lie
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    kpiece[i] = key_row * 128 + (((2 * i + hh) ^ ((key_row >> 1) & 7)) * 16);
+    vpiece[i] = n * 128 + (((2 * i + hh) ^ ((n >> 1) & 7)) * 16);
+  }
+}
+
+// Row m's part, or its output.
+template <typename T>
+__device__ inline void tile_end(const TileState<T>& w, const SharedArgs& a, const Item& it, int m, bool mine, int hh,
+                                float sum) {
+  if (!mine) return;
+  T* dst = nullptr;
+  const float inv = row_out<T>(a, it, m, w.mx, sum, hh == 0, &dst);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = w.o[i >> 2][4 * (i & 3) + e];
+    put4<T>(a, it, m, 32 * (i >> 2) + 8 * (i & 3) + 4 * hh, x, inv, dst);
+  }
+}
+
+// Values of a tile's V^T in LDS at keys `valid` and beyond become zero: all threads, four a channel.
+template <typename T>
+__device__ inline void drop_keys(char* vt, int valid) {
+  typedef typename Mma<T>::v8 v8;
+  const int r = threadIdx.x >> 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = 2 * (threadIdx.x & 3) + i, k0 = 8 * (c ^ ((r >> 1) & 7));
+    v8* const at = reinterpret_cast<v8*>(vt + r * 128 + c * 16);
+    if (k0 + 8 > valid) *at = drop_behind(*at, k0, valid);
+  }
+}
+
 // WK tiles a round: with 2, waves 0..3 work on the first and waves 4..7 on the second, on the same 128
 // rows; with 1, all eight on one tile and 256 rows.
 template <typename T, int WK, bool OWN>
@@ -833,40 +906,18 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
   row_of(a, m, b, l, gh);
   const int lim = OWN ? keys_seen(it, l) : it.n_keys;
   TileState<T> w;
-  {
-    const T* p = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_st +
-                 (int64_t)(it.h * a.group + gh) * a.q_sh + hh * 8;
-#pragma unroll
-    for (int st = 0; st < 8; ++st) w.q[st] = *reinterpret_cast<const v8*>(p + st * 16);
-  }
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
-  w.mx = -INFINITY;
-  w.sum = 0.0f;
-  const int key_row = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
-  // loads: lane (r, c) of a wave takes row r of its 8, piece c ^ (row / 2) % 8
-  const int from = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
-  const int klane = ((lane >> 3) * kHeadDim + from * 8) * 2, vlane = ((lane >> 3) * src.Tp + from * 8) * 2;
-  // operand reads: where pieces 2 i + hh of the lane's K row and V^T row lie
-  int kpiece[4], vpiece[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    kpiece[i] = key_row * 128 + (((2 * i + hh) ^ ((key_row >> 1) & 7)) * 16);
-    vpiece[i] = n * 128 + (((2 * i + hh) ^ ((n >> 1) & 7)) * 16);
-  }
+  tile_begin(w, a, it, m, hh);
+  int klane, vlane, kpiece[4], vpiece[4];
+  tile_lanes(src, wave, lane, klane, vlane, kpiece, vpiece);
   const int64_t head_size = (int64_t)src.Tp * kHeadDim;
   TileAt ring[kRing - WK];  // the tiles in use and those on their way
   auto stage = [&](TileAt& x, int t) {
     if (t == 0) walk.first();
     else walk.next();
     x = walk.at(src, it, a.heads, head_size);
-    // The address goes in as a number that hipcc cannot trace to `lds`: where it can, it waits for every
-    // load under way ahead of the round's first read (7 to 14% of a tile's time); the waits are counted below.
-    uint32_t to = (uint32_t)(uintptr_t)(lds_char*)lds + (t & (kRing - 1)) * 32 * kBlock;
-    asm volatile("" : "+s"(to));
-    stage_tile<T>(src, x, klane, vlane, (lds_char*)(uintptr_t)to, wave);
+    lds_char* const to = load_target(lds + (t & (kRing - 1)) * 32 * kBlock);
+    stage_k<T>(src, x, klane, to, wave);
+    stage_v<T>(src, x, vlane, to + 16 * kBlock, wave);
   };
 #pragma unroll
   for (int i = 0; i < kRing - WK; ++i) {
@@ -917,7 +968,7 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
       }
       v8 p[4];
       const float sum = probs<T>(sc, a.c, w.mx == -INFINITY ? 0.0f : w.mx, p);
-      settle<T>(w, sc, a.c, sum, p);
+      settle<T>(w, sc, a.c, sum, p, !(sum <= 256.0f) || w.mx == -INFINITY);
       if (masked) {
         masked_pv<T, OWN>(w, cur, partial, vt, vpiece, p);
       } else {
@@ -949,18 +1000,198 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
 #pragma unroll
     for (int i = 0; i < 64; ++i) w.o[i >> 4][i & 15] = w.o[i >> 4][i & 15] * x + at[i * 64] * y;
   }
-  if (!mine) return;
-  T* dst = nullptr;
-  const float inv = row_out<T>(a, it, m, w.mx, sum, hh == 0, &dst);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    f32x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = w.o[i >> 2][4 * (i & 3) + e];
-    put4<T>(a, it, m, 32 * (i >> 2) + 8 * (i & 3) + 4 * hh, x, inv, dst);
-  }
+  tile_end(w, a, it, m, mine, hh, sum);
 }
 
+
+// 256 rows against a prefix, software-pipelined: round t holds the scores of tile t + 1, the probabilities
+// of tile t and the second product of tile t - 1, 32 products with a slice of the softmax after each, so
+// that the matrix cores and the vector units work at the same time.  K and V have rings of their own:
+// K t + 1 and V t - 1 are in use while K t + 2 .. t + 4 and V t .. t + 2 are on their way.
+template <typename T>
+__device__ inline void prefix_item(const SharedArgs& a, const Source& src, const Item& it, char* lds) {
+  typedef typename Mma<T>::v8 v8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hh = lane >> 5;
+  const int per_page = (src.T + kTile - 1) / kTile;
+  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
+  const int t0 = share_of(n_tiles, it.split, it.n_split), n_own = share_of(n_tiles, it.split + 1, it.n_split) - t0;
+  TileWalk kw, vw;
+  if (n_own > 0) {
+    kw.start(it, per_page, t0);
+    vw.start(it, per_page, t0);
+  }
+  const bool busy = it.m0 + 32 * wave < it.m1, mine = it.m0 + 32 * wave + n < it.m1;
+  const int m = all_rows(a, it, mine ? it.m0 + 32 * wave + n : it.m0);
+  TileState<T> w;
+  tile_begin(w, a, it, m, hh);
+  int klane, vlane, kpiece[4], vpiece[4];
+  tile_lanes(src, wave, lane, klane, vlane, kpiece, vpiece);
+  const int64_t head_size = (int64_t)src.Tp * kHeadDim;
+  char* const vlds = lds + kRing * 16 * kBlock;
+  int valid[kRing + 2];  // keys of tiles t - 1 .. t + 4 of round t
+#pragma unroll
+  for (int i = 0; i < kRing + 2; ++i) valid[i] = kTile;
+  auto load_k = [&](int t) __attribute__((always_inline)) {
+    if (t == 0) kw.first();
+    else kw.next();
+    const TileAt x = kw.at(src, it, a.heads, head_size);
+    stage_k<T>(src, x, klane, load_target(lds + (t & (kRing - 1)) * 16 * kBlock), wave);
+    return x.valid;
+  };
+  auto load_v = [&](int t) __attribute__((always_inline)) {
+    if (t == 0) vw.first();
+    else vw.next();
+    stage_v<T>(src, vw.at(src, it, a.heads, head_size), vlane, load_target(vlds + (t & (kRing - 1)) * 16 * kBlock), wave);
+  };
+#pragma unroll
+  for (int i = 0; i < kRing; ++i) {
+    if (i < n_own) valid[i + 1] = load_k(i);
+    if (i >= 2 && i - 2 < n_own) load_v(i - 2);
+  }
+  // round 0 multiplies the tile in front of the first by nothing
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<u32x4*>(vlds + (kRing - 1) * 16 * kBlock + (threadIdx.x + i * 64 * kWaves) * 16) = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
+  auto mask = [&](f32x16 (&sc)[2], int keys) __attribute__((always_inline)) {
+    int most = keys - 8 * hh;
+    asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (16 * kk + i >= most) sc[kk >> 1][8 * (kk & 1) + i] = -INFINITY;
+  };
+  f32x16 sa[2], sb[2], zero;
+  v8 pa[4], pb[4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pa[i][e] = (T)0.0f;
+  if (n_own > 0) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sa[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(lds + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
+                                w.q[i >> 1], i < 2 ? zero : sa[i & 1]);
+      if (valid[1] < kTile) mask(sa, valid[1]);
+      float top = sa[0][0];  // the running maximum starts at the first tile's
+#pragma unroll
+      for (int i = 1; i < 32; ++i) top = fmaxf(top, sa[i >> 4][i & 15]);
+      w.mx = over_groups_max(top, 32) * a.c;
+    }
+  }
+  auto round = [&](int t, f32x16 (&cur)[2], f32x16 (&nxt)[2], v8 (&pprev)[4], v8 (&p)[4]) __attribute__((always_inline)) {
+    // K t + 1 and V t - 1 have landed (a wave's loads land in order; what was issued behind them may be
+    // under way), and everybody is done with K t and V t - 2, whose places load next
+    if (t + 3 < n_own) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if (t + 2 < n_own) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    else if (t + 1 < n_own) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    char* const vt = vlds + ((t - 1) & (kRing - 1)) * 16 * kBlock;
+    if (valid[0] < kTile) {  // the same for all waves
+      drop_keys<T>(vt, valid[0]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+    const char* const kt = lds + ((t + 1) & (kRing - 1)) * 16 * kBlock;
+    const int now_next = valid[2];
+#pragma unroll
+    for (int i = 0; i <= kRing; ++i) valid[i] = valid[i + 1];
+    if (t + kRing < n_own) valid[kRing] = load_k(t + kRing);
+    if (t + 2 < n_own) load_v(t + 2);
+    if (!busy) return;
+    // product i: even ones score, odd ones add values
+    auto operand = [&](int i) __attribute__((always_inline)) {
+      const int st = i >> 1;
+      return (i & 1) == 0 ? *reinterpret_cast<const v8*>(kt + kpiece[(st >> 1) & 3] + ((st >> 3) * 8 + (st & 1) * 4) * kBlock)
+                          : *reinterpret_cast<const v8*>(vt + vpiece[st >> 2] + (st & 3) * 4 * kBlock);
+    };
+    v8 ahead[4];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) ahead[i] = operand(i);
+    const float ms = w.mx == -INFINITY ? 0.0f : w.mx;
+    float e[32], part[4], sum = 0.0f;
+    bool odd = false;
+    auto expo = [&](int i) __attribute__((always_inline)) {
+      e[i] = __builtin_amdgcn_exp2f(cur[i >> 4][i & 15] * a.c - ms);
+      asm volatile("" ::"v"(e[i]));  // stays behind its product
+    };
+    auto retire = [&](int i) __attribute__((always_inline)) {
+      part[i & 3] = i < 4 ? e[i] : part[i & 3] + e[i];
+      asm volatile("" ::"v"(part[i & 3]));
+      p[i >> 3][i & 7] = (T)e[i];  // rounded to the pool's type; the sum is of fp32 values
+      if ((i & 7) == 7) asm volatile("" ::"v"(p[i >> 3]));
+    };
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if (i + 3 < 32) ahead[(i + 3) & 3] = operand(i + 3);
+      if (i == 0) __builtin_amdgcn_s_setprio(2);
+      if (i == 11) __builtin_amdgcn_s_setprio(1);
+      if (i == 22) __builtin_amdgcn_s_setprio(0);
+      const int st = i >> 1;
+      if ((i & 1) == 0) nxt[st & 1] = Mma<T>::mul(ahead[i & 3], w.q[st >> 1], st < 2 ? zero : nxt[st & 1]);
+      else w.o[st & 3] = Mma<T>::mul(ahead[i & 3], pprev[st >> 2], w.o[st & 3]);
+      // two probabilities after each of the first products, one after the others; a probability is
+      // summed and packed a product later than it is formed
+      if (i >= 1 && i <= 4) {
+        retire(2 * (i - 1));
+        retire(2 * (i - 1) + 1);
+      } else if (i >= 5 && i <= 28) {
+        retire(i + 3);
+      }
+      if (i < 4) {
+        expo(2 * i);
+        expo(2 * i + 1);
+      } else if (i < 28) {
+        expo(i + 4);
+      }
+      if (i == 30) {
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
+        odd = !(sum <= 256.0f) || w.mx == -INFINITY;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    settle<T>(w, cur, a.c, sum, p, odd);
+    if (t + 1 < n_own && now_next < kTile) mask(nxt, now_next);
+  };
+  int t = 0;
+  for (; t + 1 < n_own; t += 2) {
+    round(t, sa, sb, pa, pb);
+    round(t + 1, sb, sa, pb, pa);
+  }
+  if (t < n_own) round(t, sa, sb, pa, pb);
+  if (n_own > 0) {  // the last tile's second product
+    const int last = n_own - 1;
+    char* const vt = vlds + (last & (kRing - 1)) * 16 * kBlock;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (valid[0] < kTile) {
+      drop_keys<T>(vt, valid[0]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        w.o[i & 3] = Mma<T>::mul(*reinterpret_cast<const v8*>(vt + vpiece[i >> 2] + (i & 3) * 4 * kBlock),
+                                 n_own & 1 ? pb[i >> 2] : pa[i >> 2], w.o[i & 3]);
+    }
+  }
+  tile_end(w, a, it, m, mine, hh, over_groups_sum(w.sum, 32));
+}
 
 __device__ inline void prefix_keys(const SharedArgs& a, Item& it) {
   it.list = a.pre_pages;
@@ -1048,7 +1279,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
     it.m0 = rb * R;
     it.m1 = it.m0 + R < rows ? it.m0 + R : rows;
     prefix_keys(a, it);
-    if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
+    if constexpr (PK == 1) prefix_item<T>(a, a.pre, it, lds);
+    else if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
     else stream_item<T, false>(a, a.pre, it, kWaves, reinterpret_cast<float*>(lds));
     return;
   }
