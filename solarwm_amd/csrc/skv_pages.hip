@@ -877,10 +877,12 @@ __device__ inline void tile_end(const TileState<T>& w, const SharedArgs& a, cons
 template <typename T>
 __device__ inline void drop_keys(char* vt, int valid) {
   typedef typename Mma<T>::v8 v8;
-  const int r = threadIdx.x >> 2;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // nothing of this is worth registers in the loop around it
+  const int r = tid >> 2;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int c = 2 * (threadIdx.x & 3) + i, k0 = 8 * (c ^ ((r >> 1) & 7));
+    const int c = 2 * (tid & 3) + i, k0 = 8 * (c ^ ((r >> 1) & 7));
     v8* const at = reinterpret_cast<v8*>(vt + r * 128 + c * 16);
     if (k0 + 8 > valid) *at = drop_behind(*at, k0, valid);
   }
@@ -1056,8 +1058,9 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
 #pragma unroll
   for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
   auto mask = [&](f32x16 (&sc)[2], int keys) __attribute__((always_inline)) {
-    int most = keys - 8 * hh;
-    asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // keeps this a branch: most tiles have nothing to mask
+    const int most = keys - ((tid & 32) >> 2);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
