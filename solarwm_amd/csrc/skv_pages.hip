@@ -234,7 +234,7 @@ struct SharedArgs {
   int batch, rows, heads, group, causal;
   float c;       // softmax_scale * log2(e)
   int M;         // batch * rows * group
-  int pre_rb, pre_splits, pre_grid;  // row blocks, key splits and workgroups of the prefix
+  int pre_splits, pre_grid;  // key splits and workgroups of the prefix
   int own_rb, own_splits, own_items, own_waves;  // row blocks of a sequence, key splits; waves of an item
   int direct;    // one part only: workgroups write out themselves
   int both;      // (direct) one sequence, few rows: prefix and own keys in one work item
@@ -1244,15 +1244,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
     }
   }
   if ((int)blockIdx.x < a.pre_grid) {
-    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
     constexpr int R = kind_rows(PK);
-    // a padded batch's last row blocks may hold no tokens: they come last
-    const int per = a.pre_grid / 8 / a.pre_rb, pair = (a.new_lens ? at % per : at / a.pre_rb) * 8 + xcd;
-    const int rb = a.new_lens ? at / per : at % a.pre_rb;
-    if (pair >= a.heads * a.pre_splits) return;
-    it.h = pair % a.heads;
-    it.split = it.part = pair / a.heads;
-    it.n_split = a.pre_splits;
     int rows = a.M;
     it.tokens = nullptr;
     if constexpr (PK) {
@@ -1276,10 +1268,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
         __syncthreads();
         it.tokens = tokens;
         rows = __builtin_amdgcn_readfirstlane(tokens[a.batch]) * a.group;
-        if (rb * R >= rows) return;
       }
     }
-    it.m0 = rb * R;
+    // every eighth workgroup runs on the same XCD: each gets an equal run of (key head, split)s' row blocks
+    const int blocks = (rows + R - 1) / R, n = a.heads * a.pre_splits * blocks, each = (n + 7) / 8;
+    const int at = blockIdx.x >> 3, unit = (blockIdx.x & 7) * each + at;
+    if (at >= each || unit >= n) return;
+    const int pair = unit / blocks;
+    it.h = pair % a.heads;
+    it.split = it.part = pair / a.heads;
+    it.n_split = a.pre_splits;
+    it.m0 = (unit - pair * blocks) * R;
     it.m1 = it.m0 + R < rows ? it.m0 + R : rows;
     prefix_keys(a, it);
     if constexpr (PK == 1) prefix_item<T>(a, a.pre, it, lds);
@@ -1419,22 +1418,22 @@ int common_errors(const char* fn, int dtype, int head_dim, int batch, int rows, 
 struct SharedPlan {
   int pre_kind, own_kind;
   bool both;  // one sequence with few rows and keys: a head's prefix and own keys in one work item
-  int pre_rb, pre_splits, pre_grid, own_rb, own_splits, own_items, own_waves, own_grid, parts;
+  int pre_splits, pre_grid, own_rb, own_splits, own_items, own_waves, own_grid, parts;
   int64_t bytes;
 };
 
 // Key splits, and waves of a streaming item, by what they are estimated to take (microseconds, as
 // measured on MI355X).  A workgroup has a CU to itself, so what counts is rounds of workgroups.  A
-// workgroup takes kFixed to start and end (7.5 us with two steps); a tile of 256 rows 1.7 us with up to
-// two thirds of the CUs busy and 2.2 with all (the clock follows the power), two tiles of 128 rows 2.3; a
-// streaming CU reads 38 GB/s (64 keys in 0.86 us), and the whole chip 4.6 TB/s.  Every part costs its
-// partial results and the merge.
+// workgroup takes kFixed to start and end (7.5 us with two steps).  A tile against 256 rows takes 1.45 us
+// of a prefix and 1.7 of own pages while half of the CUs work, and 2.0 and 2.2 when all do (the clock
+// follows the power), two tiles against 128 rows 2.3.  A streaming CU reads 38 GB/s (64 keys in 0.86 us),
+// and the whole chip 4.6 TB/s.  Several parts cost kMerge and the bytes of their partial results.
 void choose_splits(const skv_attend_shared_desc* d, int64_t M, int64_t cu, int64_t pre_items, int64_t pre_tiles,
                    int64_t own_items, int64_t own_tiles, SharedPlan* p) {
   constexpr double kFixed = 7.0, kBytes = 4.6e6, kMerge = 7.0, kTileBytes = 32768.0;
-  auto tile_cost = [](int kind, double busy) {
-    const double over = (busy < 1.0 ? busy : 1.0) - 0.65;
-    return kind == 0 ? 0.86 : kind == 2 ? 1.15 : 1.7 + (over > 0 ? 1.4 * over : 0.0);
+  auto tile_cost = [](int kind, bool own, double busy) {
+    const double over = busy < 0.5 ? 0.0 : (busy < 1.0 ? busy : 1.0) - 0.5;
+    return kind == 0 ? 0.86 : kind == 2 ? 1.15 : own ? 1.7 + over : 1.45 + 1.1 * over;
   };
   // tables are as wide as their longest sequence gets: the average one holds half of that
   const double mean = 0.5 * own_tiles, longer = 0.75 * own_tiles;
@@ -1459,8 +1458,8 @@ void choose_splits(const skv_attend_shared_desc* d, int64_t M, int64_t cu, int64
       }
       const int64_t n_pre = pre_items * ps, full = n_pre / cu, part = n_pre % cu;
       const double busy = (double)(full ? cu : part) / cu;
-      const double dp = ps ? kFixed + (double)((pre_tiles + ps - 1) / ps) * tile_cost(p->pre_kind, busy) : 0.0;
-      const double dn = kFixed + longer / os * tile_cost(p->own_kind, (double)n_own / cu) * kWaves / waves;
+      const double dp = ps ? kFixed + (double)((pre_tiles + ps - 1) / ps) * tile_cost(p->pre_kind, false, busy) : 0.0;
+      const double dn = kFixed + longer / os * tile_cost(p->own_kind, true, (double)n_own / cu) * kWaves / waves;
       double t;
       if (n_pre + n_own <= cu) {
         t = n_own && dn > dp ? dn : dp;
@@ -1502,12 +1501,12 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
   };
   const int64_t pre_tiles = pre ? tiles(d->prefix_tokens, d->prefix_page_tokens) : 0;
   const int64_t own_tiles = own ? tiles((int64_t)d->table_width * d->page_tokens, d->page_tokens) : 0;
-  p->pre_rb = pre ? (int)((M + pre_rows - 1) / pre_rows) : 0;
+  const int64_t pre_rb = pre ? (M + pre_rows - 1) / pre_rows : 0;
   p->own_rb = own ? (int)((per + own_rows - 1) / own_rows) : 0;
-  const int64_t pre_items = (int64_t)p->pre_rb * d->kv_heads;
+  const int64_t pre_items = pre_rb * d->kv_heads;
   const int64_t own_items = (int64_t)p->own_rb * d->kv_heads * d->batch;
   // of a padded batch's row blocks about half hold tokens
-  const int64_t busy_rb = d->new_lens && p->pre_kind ? (M / 2 + pre_rows) / pre_rows : p->pre_rb;
+  const int64_t busy_rb = d->new_lens && p->pre_kind ? (M / 2 + pre_rows) / pre_rows : pre_rb;
   // A sequence by itself with few rows and keys needs no second part and no merge (12.1 us for 390 + 64
   // keys of 12 heads, and 15.3 in two parts); in several parts its own keys are better off beside the
   // prefix (19.6 us for 8190 + 1560 keys of 8 heads, and 22.3 in one list).
@@ -1516,10 +1515,10 @@ int plan_shared(const char* fn, const skv_attend_shared_desc* d, SharedPlan* p) 
     p->both = p->pre_splits == 1;
   }
   if (!p->both)
-    choose_splits(d, M, cu, busy_rb < p->pre_rb ? busy_rb * d->kv_heads : pre_items, pre_tiles, own_items, own_tiles, p);
+    choose_splits(d, M, cu, busy_rb < pre_rb ? busy_rb * d->kv_heads : pre_items, pre_tiles, own_items, own_tiles, p);
   p->parts = p->pre_splits + p->own_splits;
-  const int64_t pairs = (int64_t)d->kv_heads * p->pre_splits, each = p->own_kind ? 1 : kWaves / p->own_waves;
-  const int64_t pre_grid = (pairs + 7) / 8 * 8 * p->pre_rb, all_own = own_items * p->own_splits;
+  const int64_t each = p->own_kind ? 1 : kWaves / p->own_waves;
+  const int64_t pre_grid = (pre_items * p->pre_splits + 7) / 8 * 8, all_own = own_items * p->own_splits;
   if ((pre_grid + (all_own + each - 1) / each) * 64 * kWaves >= kMaxThreads) {
     set_error("%s: too many work items", fn);
     return SKV_E_ARG;
@@ -1713,7 +1712,7 @@ extern "C" int skv_attend_shared(const skv_attend_shared_desc* d, skv_stream_t s
   a.batch = d->batch, a.rows = d->rows, a.heads = d->kv_heads, a.group = d->q_heads / d->kv_heads;
   a.causal = d->causal != 0, a.c = d->softmax_scale * 1.44269504088896340736f;
   a.M = d->batch * d->rows * a.group;
-  a.pre_rb = p.pre_rb, a.pre_splits = p.pre_splits, a.pre_grid = p.pre_grid;
+  a.pre_splits = p.pre_splits, a.pre_grid = p.pre_grid;
   a.own_rb = p.own_rb, a.own_splits = p.own_splits;
   a.own_items = p.own_items, a.own_waves = p.own_waves;
   a.direct = p.parts == 1, a.both = p.both;
