@@ -5,6 +5,8 @@
 // tokens of a page in use (Tp = T rounded up to 64).  A sequence's token i lies at offset i % T of
 // page tables[b][i / T]; page numbers outside the pool are pages that are not there: nothing is
 // written to them and their keys are not seen.
+#include <utility>
+
 #include "skv_rowops.h"
 
 namespace skv {
@@ -1006,6 +1008,19 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
 }
 
 
+// Scores of keys `most` and beyond (of a lane's 32: register i is key 16 (i / 8) + i % 8) become -infinity.
+// A compare and a choice each: as plain code hipcc makes all 32 comparisons first and spills them.
+template <int KEY>
+__device__ inline float unless_seen(float x, int most, float none) {
+  asm("v_cmp_lt_i32 vcc, %2, %1\n\tv_cndmask_b32 %0, %3, %0, vcc" : "+v"(x) : "v"(most), "n"(KEY), "v"(none) : "vcc");
+  return x;
+}
+template <int... I>
+__device__ inline void mask_keys(f32x16 (&sc)[2], int most, std::integer_sequence<int, I...>) {
+  const float none = -INFINITY;
+  ((sc[I >> 4][I & 15] = unless_seen<16 * (I / 8) + I % 8>(sc[I >> 4][I & 15], most, none)), ...);
+}
+
 // 256 rows against a prefix, software-pipelined: round t holds the scores of tile t + 1, the probabilities
 // of tile t and the second product of tile t - 1, 32 products with a slice of the softmax after each, so
 // that the matrix cores and the vector units work at the same time.  K and V have rings of their own:
@@ -1031,9 +1046,7 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
   tile_lanes(src, wave, lane, klane, vlane, kpiece, vpiece);
   const int64_t head_size = (int64_t)src.Tp * kHeadDim;
   char* const vlds = lds + kRing * 16 * kBlock;
-  int valid[kRing + 2];  // keys of tiles t - 1 .. t + 4 of round t
-#pragma unroll
-  for (int i = 0; i < kRing + 2; ++i) valid[i] = kTile;
+  int valid[kRing];  // keys of tiles t .. t + 3 at round t
   auto load_k = [&](int t) __attribute__((always_inline)) {
     if (t == 0) kw.first();
     else kw.next();
@@ -1048,7 +1061,8 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
   };
 #pragma unroll
   for (int i = 0; i < kRing; ++i) {
-    if (i < n_own) valid[i + 1] = load_k(i);
+    valid[i] = kTile;
+    if (i < n_own) valid[i] = load_k(i);
     if (i >= 2 && i - 2 < n_own) load_v(i - 2);
   }
   // round 0 multiplies the tile in front of the first by nothing
@@ -1061,11 +1075,7 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // keeps this a branch: most tiles have nothing to mask
     const int most = keys - ((tid & 32) >> 2);
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (16 * kk + i >= most) sc[kk >> 1][8 * (kk & 1) + i] = -INFINITY;
+    mask_keys(sc, most, std::make_integer_sequence<int, 32>{});
   };
   f32x16 sa[2], sb[2], zero;
   v8 pa[4], pb[4];
@@ -1084,7 +1094,7 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
       for (int i = 0; i < 16; ++i)
         sa[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(lds + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
                                 w.q[i >> 1], i < 2 ? zero : sa[i & 1]);
-      if (valid[1] < kTile) mask(sa, valid[1]);
+      if (valid[0] < kTile) mask(sa, valid[0]);
       float top = sa[0][0];  // the running maximum starts at the first tile's
 #pragma unroll
       for (int i = 1; i < 32; ++i) top = fmaxf(top, sa[i >> 4][i & 15]);
@@ -1094,24 +1104,25 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
   auto round = [&](int t, f32x16 (&cur)[2], f32x16 (&nxt)[2], v8 (&pprev)[4], v8 (&p)[4]) __attribute__((always_inline)) {
     // K t + 1 and V t - 1 have landed (a wave's loads land in order; what was issued behind them may be
     // under way), and everybody is done with K t and V t - 2, whose places load next
-    if (t + 3 < n_own) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    else if (t + 2 < n_own) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-    else if (t + 1 < n_own) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+    const bool cut = valid[0] < kTile;  // tile t, the same for all waves: V t too, to lose what is no key
+    if (t + 3 < n_own) {
+      if (cut) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else if (cut || t + 1 >= n_own) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    char* const vt = vlds + ((t - 1) & (kRing - 1)) * 16 * kBlock;
-    if (valid[0] < kTile) {  // the same for all waves
-      drop_keys<T>(vt, valid[0]);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-    }
+    if (cut) drop_keys<T>(vlds + (t & (kRing - 1)) * 16 * kBlock, valid[0]);
+    const char* const vt = vlds + ((t - 1) & (kRing - 1)) * 16 * kBlock;
     const char* const kt = lds + ((t + 1) & (kRing - 1)) * 16 * kBlock;
-    const int now_next = valid[2];
+    const int next_valid = valid[1];
 #pragma unroll
-    for (int i = 0; i <= kRing; ++i) valid[i] = valid[i + 1];
-    if (t + kRing < n_own) valid[kRing] = load_k(t + kRing);
+    for (int i = 0; i + 1 < kRing; ++i) valid[i] = valid[i + 1];
+    if (t + kRing < n_own) valid[kRing - 1] = load_k(t + kRing);
     if (t + 2 < n_own) load_v(t + 2);
     if (!busy) return;
     // product i: even ones score, odd ones add values
@@ -1166,7 +1177,7 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
       __builtin_amdgcn_sched_barrier(0);
     }
     settle<T>(w, cur, a.c, sum, p, odd);
-    if (t + 1 < n_own && now_next < kTile) mask(nxt, now_next);
+    if (t + 1 < n_own && next_valid < kTile) mask(nxt, next_valid);
   };
   int t = 0;
   for (; t + 1 < n_own; t += 2) {
@@ -1176,16 +1187,10 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
   if (t < n_own) round(t, sa, sb, pa, pb);
   if (n_own > 0) {  // the last tile's second product
     const int last = n_own - 1;
-    char* const vt = vlds + (last & (kRing - 1)) * 16 * kBlock;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const char* const vt = vlds + (last & (kRing - 1)) * 16 * kBlock;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (valid[0] < kTile) {
-      drop_keys<T>(vt, valid[0]);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-    }
     if (busy) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
