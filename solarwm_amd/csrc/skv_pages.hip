@@ -775,6 +775,19 @@ __device__ inline void settle(TileState<T>& w, const f32x16 (&sc)[2], float c, f
   w.sum += sum;
 }
 
+// Scores of keys `most` and beyond (of a lane's 32: register i is key 16 (i / 8) + i % 8) become -infinity.
+// A compare and a choice each: as plain code hipcc makes all 32 comparisons first and spills them.
+template <int KEY>
+__device__ inline float unless_seen(float x, int most, float none) {
+  asm("v_cmp_lt_i32 vcc, %2, %1\n\tv_cndmask_b32 %0, %3, %0, vcc" : "+v"(x) : "v"(most), "n"(KEY), "v"(none) : "vcc");
+  return x;
+}
+template <int... I>
+__device__ inline void mask_keys(f32x16 (&sc)[2], int most, std::integer_sequence<int, I...>) {
+  const float none = -INFINITY;
+  ((sc[I >> 4][I & 15] = unless_seen<16 * (I / 8) + I % 8>(sc[I >> 4][I & 15], most, none)), ...);
+}
+
 // The second product of a tile that has keys which do not exist, or (OWN) that some rows do not see.
 template <typename T, bool OWN>
 __device__ inline void masked_pv(TileState<T>& w, const TileAt& x, bool partial, const char* vt,
@@ -962,13 +975,7 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
         const int seen = lim - cur.key0;
         int most = (seen < cur.valid ? seen : cur.valid) - 8 * hh;
         asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if (!partial && 16 * kk + 16 <= cur.valid) continue;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (16 * kk + i >= most) sc[kk >> 1][8 * (kk & 1) + i] = -INFINITY;
-        }
+        mask_keys(sc, most, std::make_integer_sequence<int, 32>{});
       }
       v8 p[4];
       const float sum = probs<T>(sc, a.c, w.mx == -INFINITY ? 0.0f : w.mx, p);
@@ -1007,19 +1014,6 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
   tile_end(w, a, it, m, mine, hh, sum);
 }
 
-
-// Scores of keys `most` and beyond (of a lane's 32: register i is key 16 (i / 8) + i % 8) become -infinity.
-// A compare and a choice each: as plain code hipcc makes all 32 comparisons first and spills them.
-template <int KEY>
-__device__ inline float unless_seen(float x, int most, float none) {
-  asm("v_cmp_lt_i32 vcc, %2, %1\n\tv_cndmask_b32 %0, %3, %0, vcc" : "+v"(x) : "v"(most), "n"(KEY), "v"(none) : "vcc");
-  return x;
-}
-template <int... I>
-__device__ inline void mask_keys(f32x16 (&sc)[2], int most, std::integer_sequence<int, I...>) {
-  const float none = -INFINITY;
-  ((sc[I >> 4][I & 15] = unless_seen<16 * (I / 8) + I % 8>(sc[I >> 4][I & 15], most, none)), ...);
-}
 
 // 256 rows against a prefix, software-pipelined: round t holds the scores of tile t + 1, the probabilities
 // of tile t and the second product of tile t - 1, 32 products with a slice of the softmax after each, so
