@@ -1308,6 +1308,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
   else stream_item<T, true>(a, a.own, it, waves, reinterpret_cast<float*>(lds));
 }
 
+// The join of up to kFewParts parts: half a wave per (row, key head), a lane four channels, all parts'
+// values under way at once.
+constexpr int kFewParts = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void merge_few_kernel(SharedArgs a, int n_parts) {
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int c = 4 * (threadIdx.x & 31);
+  if (unit >= (int64_t)a.heads * a.M) return;
+  const int h = (int)(unit % a.heads), m = (int)(unit / a.heads);
+  int b, l, gh;
+  row_of(a, m, b, l, gh);
+  const int64_t at = (int64_t)h * a.M + m, step = (int64_t)a.heads * a.M;
+  f32x4 v[kFewParts], o = f32x4{0.f, 0.f, 0.f, 0.f};
+  float2 ml[kFewParts];
+#pragma unroll
+  for (int p = 0; p < kFewParts; ++p) {
+    if (p >= n_parts) break;
+    ml[p] = a.part_ml[at + p * step];
+    v[p] = *reinterpret_cast<const f32x4*>(a.part_o + (at + p * step) * kHeadDim + c);
+  }
+  float top = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (int p = 0; p < kFewParts; ++p)
+    if (p < n_parts) top = fmaxf(top, ml[p].x);
+  if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+  for (int p = 0; p < kFewParts; ++p)
+    if (p < n_parts) {
+      const float x = __builtin_amdgcn_exp2f(ml[p].x - top);
+      total += x * ml[p].y;
+      o += x * v[p];
+    }
+  const bool any = l < fresh_rows(a, b) && total != 0.0f;  // a row that sees no key is zero (NaN sums are not zero)
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = any ? (T)(o[i] / total) : (T)0.0f;
+  *reinterpret_cast<t4*>(static_cast<T*>(a.out) + b * a.o_sb + l * a.o_st + (int64_t)(h * a.group + gh) * a.o_sh + c) = r;
+}
+
 // One wave per (row, key head).  Lane p weighs part p (64 parts at a time); then each half of the wave
 // adds every other part, a lane four channels, with four loads in flight.
 template <typename T>
@@ -1575,6 +1615,14 @@ void launch_shared(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
   else launch(attend_shared_kernel<T, 1, 1>);
 }
 
+template <typename T>
+void launch_merge(const SharedArgs& a, int parts, hipStream_t s) {
+  const int each = parts <= kFewParts ? 8 : 4;
+  const dim3 grid((unsigned)(((int64_t)a.heads * a.M + each - 1) / each)), block(256);
+  if (parts <= kFewParts) hipLaunchKernelGGL(merge_few_kernel<T>, grid, block, 0, s, a, parts);
+  else hipLaunchKernelGGL(merge_kernel<T>, grid, block, 0, s, a, parts);
+}
+
 }  // namespace
 
 }  // namespace skv
@@ -1724,8 +1772,7 @@ extern "C" int skv_attend_shared(const skv_attend_shared_desc* d, skv_stream_t s
     st = launched(fn);
     if (st != SKV_OK || a.direct) return st;
   }
-  const dim3 grid((unsigned)(((int64_t)a.heads * a.M + 3) / 4)), block(256);
-  if (d->dtype == SKV_BF16) hipLaunchKernelGGL(merge_kernel<bf16>, grid, block, 0, s, a, p.parts);
-  else hipLaunchKernelGGL(merge_kernel<f16>, grid, block, 0, s, a, p.parts);
+  if (d->dtype == SKV_BF16) launch_merge<bf16>(a, p.parts, s);
+  else launch_merge<f16>(a, p.parts, s);
   return launched(fn);
 }
