@@ -782,10 +782,15 @@ __device__ inline float unless_seen(float x, int most, float none) {
   asm("v_cmp_lt_i32 vcc, %2, %1\n\tv_cndmask_b32 %0, %3, %0, vcc" : "+v"(x) : "v"(most), "n"(KEY), "v"(none) : "vcc");
   return x;
 }
-template <int... I>
-__device__ inline void mask_keys(f32x16 (&sc)[2], int most, std::integer_sequence<int, I...>) {
+template <int KK, int... I>
+__device__ inline void mask_eight(f32x16& sc, int most, std::integer_sequence<int, I...>) {
   const float none = -INFINITY;
-  ((sc[I >> 4][I & 15] = unless_seen<16 * (I / 8) + I % 8>(sc[I >> 4][I & 15], most, none)), ...);
+  ((sc[8 * (KK & 1) + I] = unless_seen<16 * KK + I>(sc[8 * (KK & 1) + I], most, none)), ...);
+}
+// `from`: keys below it need no look, the same for the whole wave
+template <int... KK>
+__device__ inline void mask_keys(f32x16 (&sc)[2], int most, int from, std::integer_sequence<int, KK...>) {
+  ((16 * KK + 16 > from ? mask_eight<KK>(sc[KK >> 1], most, std::make_integer_sequence<int, 8>{}) : void()), ...);
 }
 
 // The second product of a tile that has keys which do not exist, or (OWN) that some rows do not see.
@@ -899,7 +904,8 @@ __device__ inline void drop_keys(char* vt, int valid) {
   for (int i = 0; i < 2; ++i) {
     const int c = 2 * (tid & 3) + i, k0 = 8 * (c ^ ((r >> 1) & 7));
     v8* const at = reinterpret_cast<v8*>(vt + r * 128 + c * 16);
-    if (k0 + 8 > valid) *at = drop_behind(*at, k0, valid);
+    if (k0 >= valid) *at = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
+    else if (k0 + 8 > valid) *at = drop_behind(*at, k0, valid);
   }
 }
 
@@ -975,7 +981,7 @@ __device__ inline void tile_item(const SharedArgs& a, const Source& src, const I
         const int seen = lim - cur.key0;
         int most = (seen < cur.valid ? seen : cur.valid) - 8 * hh;
         asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
-        mask_keys(sc, most, std::make_integer_sequence<int, 32>{});
+        mask_keys(sc, most, OWN ? 0 : cur.valid, std::make_integer_sequence<int, 4>{});
       }
       v8 p[4];
       const float sum = probs<T>(sc, a.c, w.mx == -INFINITY ? 0.0f : w.mx, p);
@@ -1069,7 +1075,7 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // keeps this a branch: most tiles have nothing to mask
     const int most = keys - ((tid & 32) >> 2);
-    mask_keys(sc, most, std::make_integer_sequence<int, 32>{});
+    mask_keys(sc, most, keys, std::make_integer_sequence<int, 4>{});
   };
   f32x16 sa[2], sb[2], zero;
   v8 pa[4], pb[4];
