@@ -909,141 +909,17 @@ __device__ inline void drop_keys(char* vt, int valid) {
   }
 }
 
-// WK tiles a round: with 2, waves 0..3 work on the first and waves 4..7 on the second, on the same 128
-// rows; with 1, all eight on one tile and 256 rows.
-template <typename T, int WK, bool OWN>
-__device__ inline void tile_item(const SharedArgs& a, const Source& src, const Item& it, char* lds) {
-  typedef typename Mma<T>::v8 v8;
-  constexpr int kRows = kWaves / WK;  // waves side by side
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 31, hh = lane >> 5, wr = wave % kRows, wk = wave / kRows;
-  const int per_page = (src.T + kTile - 1) / kTile;
-  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
-  const int t0 = share_of(n_tiles, it.split, it.n_split), n_own = share_of(n_tiles, it.split + 1, it.n_split) - t0;
-  TileWalk walk;  // at the tile that loads last
-  if (n_own > 0) walk.start(it, per_page, t0);  // the page list loads while the rows are looked up
-  const bool busy = it.m0 + 32 * wr < it.m1;  // the wave has rows at all
-  const bool mine = it.m0 + 32 * wr + n < it.m1;
-  const int m = all_rows(a, it, mine ? it.m0 + 32 * wr + n : it.m0);
-  int b, l, gh;
-  row_of(a, m, b, l, gh);
-  const int lim = OWN ? keys_seen(it, l) : it.n_keys;
-  TileState<T> w;
-  tile_begin(w, a, it, m, hh);
-  int klane, vlane, kpiece[4], vpiece[4];
-  tile_lanes(src, wave, lane, klane, vlane, kpiece, vpiece);
-  const int64_t head_size = (int64_t)src.Tp * kHeadDim;
-  TileAt ring[kRing - WK];  // the tiles in use and those on their way
-  auto stage = [&](TileAt& x, int t) {
-    if (t == 0) walk.first();
-    else walk.next();
-    x = walk.at(src, it, a.heads, head_size);
-    lds_char* const to = load_target(lds + (t & (kRing - 1)) * 32 * kBlock);
-    stage_k<T>(src, x, klane, to, wave);
-    stage_v<T>(src, x, vlane, to + 16 * kBlock, wave);
-  };
-#pragma unroll
-  for (int i = 0; i < kRing - WK; ++i) {
-    ring[i] = TileAt{};
-    if (i < n_own) stage(ring[i], i);
-  }
-  // the queries' own wait, ahead of the loop's counted ones
-#pragma unroll
-  for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
-  for (int t = 0; t < n_own; t += WK) {
-    // This round's tiles have landed (a wave's loads land in order: what was issued after them may
-    // still be under way), and everybody is done with the round before, whose buffers load next.
-    constexpr int kLoads = 4;  // of a wave and tile
-    if (WK == 1 && t + 2 < n_own) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
-    else if (WK == 1 && t + 1 < n_own) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const TileAt cur = WK == 2 && wk == 1 ? ring[1] : ring[0];
-#pragma unroll
-    for (int i = 0; i + WK < kRing - WK; ++i) ring[i] = ring[i + WK];
-#pragma unroll
-    for (int i = 0; i < WK; ++i)
-      if (t + kRing - WK + i < n_own) stage(ring[kRing - 2 * WK + i], t + kRing - WK + i);
-    const char* const kt = lds + ((t + wk) & (kRing - 1)) * 32 * kBlock;
-    const char* const vt = kt + 16 * kBlock;
-    if (busy && t + wk < n_own) {
-      f32x16 sc[2];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        sc[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(kt + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
-                                w.q[i >> 1], sc[i & 1]);
-      ahead_of_products();
-      const bool partial = OWN && cur.key0 + cur.valid > it.open, masked = cur.valid < kTile || partial;
-      if (masked) {
-        const int seen = lim - cur.key0;
-        int most = (seen < cur.valid ? seen : cur.valid) - 8 * hh;
-        asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
-        mask_keys(sc, most, OWN ? 0 : cur.valid, std::make_integer_sequence<int, 4>{});
-      }
-      v8 p[4];
-      const float sum = probs<T>(sc, a.c, w.mx == -INFINITY ? 0.0f : w.mx, p);
-      settle<T>(w, sc, a.c, sum, p, !(sum <= 256.0f) || w.mx == -INFINITY);
-      if (masked) {
-        masked_pv<T, OWN>(w, cur, partial, vt, vpiece, p);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          w.o[i & 3] = Mma<T>::mul(*reinterpret_cast<const v8*>(vt + vpiece[i >> 2] + (i & 3) * 4 * kBlock), p[i >> 2],
-                                   w.o[i & 3]);
-        ahead_of_products();
-      }
-    }
-  }
-  float sum = over_groups_sum(w.sum, 32);
-  if constexpr (WK == 2) {  // the two halves of the waves join through LDS
-    float* const at = reinterpret_cast<float*>(lds) + wr * 66 * 64 + lane;
-    __syncthreads();
-    if (wk == 1) {
-#pragma unroll
-      for (int i = 0; i < 64; ++i) at[i * 64] = w.o[i >> 4][i & 15];
-      at[64 * 64] = w.mx;
-      at[65 * 64] = sum;
-    }
-    __syncthreads();
-    if (wk == 1) return;
-    const float m2 = at[64 * 64], l2 = at[65 * 64];
-    const float top = fmaxf(w.mx, m2), ms = top == -INFINITY ? 0.0f : top;
-    const float x = __builtin_amdgcn_exp2f(w.mx - ms), y = __builtin_amdgcn_exp2f(m2 - ms);
-    w.mx = top;
-    sum = sum * x + l2 * y;
-#pragma unroll
-    for (int i = 0; i < 64; ++i) w.o[i >> 4][i & 15] = w.o[i >> 4][i & 15] * x + at[i * 64] * y;
-  }
-  tile_end(w, a, it, m, mine, hh, sum);
-}
-
-
-// 256 rows against a prefix, software-pipelined: round t holds the scores of tile t + 1, the probabilities
+// 256 rows against keys that all of them see, software-pipelined: round t holds the scores of tile t + 1, the probabilities
 // of tile t and the second product of tile t - 1, 32 products with a slice of the softmax after each, so
 // that the matrix cores and the vector units work at the same time.  K and V have rings of their own:
 // K t + 1 and V t - 1 are in use while K t + 2 .. t + 4 and V t .. t + 2 are on their way.
+// Tiles [t0, t0 + n_own) of the item's keys, which all rows see as far as they exist; kw and vw have started
+// at t0.
 template <typename T>
-__device__ inline void prefix_item(const SharedArgs& a, const Source& src, const Item& it, char* lds) {
+__device__ inline __attribute__((always_inline)) void open_tiles(TileState<T>& w, TileWalk& kw, TileWalk& vw, const SharedArgs& a, const Source& src,
+                                  const Item& it, int n_own, bool busy, int wave, int klane, int vlane,
+                                  const int (&kpiece)[4], const int (&vpiece)[4], char* lds) {
   typedef typename Mma<T>::v8 v8;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 31, hh = lane >> 5;
-  const int per_page = (src.T + kTile - 1) / kTile;
-  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
-  const int t0 = share_of(n_tiles, it.split, it.n_split), n_own = share_of(n_tiles, it.split + 1, it.n_split) - t0;
-  TileWalk kw, vw;
-  if (n_own > 0) {
-    kw.start(it, per_page, t0);
-    vw.start(it, per_page, t0);
-  }
-  const bool busy = it.m0 + 32 * wave < it.m1, mine = it.m0 + 32 * wave + n < it.m1;
-  const int m = all_rows(a, it, mine ? it.m0 + 32 * wave + n : it.m0);
-  TileState<T> w;
-  tile_begin(w, a, it, m, hh);
-  int klane, vlane, kpiece[4], vpiece[4];
-  tile_lanes(src, wave, lane, klane, vlane, kpiece, vpiece);
   const int64_t head_size = (int64_t)src.Tp * kHeadDim;
   char* const vlds = lds + kRing * 16 * kBlock;
   int valid[kRing];  // keys of tiles t .. t + 3 at round t
@@ -1085,21 +961,19 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) pa[i][e] = (T)0.0f;
-  if (n_own > 0) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (busy) {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (busy) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        sa[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(lds + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
-                                w.q[i >> 1], i < 2 ? zero : sa[i & 1]);
-      if (valid[0] < kTile) mask(sa, valid[0]);
-      float top = sa[0][0];  // the running maximum starts at the first tile's
+    for (int i = 0; i < 16; ++i)
+      sa[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(lds + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
+                              w.q[i >> 1], i < 2 ? zero : sa[i & 1]);
+    if (valid[0] < kTile) mask(sa, valid[0]);
+    float top = sa[0][0];  // the running maximum starts at the first tile's
 #pragma unroll
-      for (int i = 1; i < 32; ++i) top = fmaxf(top, sa[i >> 4][i & 15]);
-      w.mx = over_groups_max(top, 32) * a.c;
-    }
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, sa[i >> 4][i & 15]);
+    w.mx = over_groups_max(top, 32) * a.c;
   }
   auto round = [&](int t, f32x16 (&cur)[2], f32x16 (&nxt)[2], v8 (&pprev)[4], v8 (&p)[4]) __attribute__((always_inline)) {
     // K t + 1 and V t - 1 have landed (a wave's loads land in order; what was issued behind them may be
@@ -1185,21 +1059,152 @@ __device__ inline void prefix_item(const SharedArgs& a, const Source& src, const
     round(t + 1, sb, sa, pb, pa);
   }
   if (t < n_own) round(t, sa, sb, pa, pb);
-  if (n_own > 0) {  // the last tile's second product
-    const int last = n_own - 1;
-    const char* const vt = vlds + (last & (kRing - 1)) * 16 * kBlock;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (busy) {
+  const int last = n_own - 1;
+  const char* const vt = vlds + (last & (kRing - 1)) * 16 * kBlock;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (busy) {  // the last tile's second product
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        w.o[i & 3] = Mma<T>::mul(*reinterpret_cast<const v8*>(vt + vpiece[i >> 2] + (i & 3) * 4 * kBlock),
-                                 n_own & 1 ? pb[i >> 2] : pa[i >> 2], w.o[i & 3]);
+    for (int i = 0; i < 16; ++i)
+      w.o[i & 3] = Mma<T>::mul(*reinterpret_cast<const v8*>(vt + vpiece[i >> 2] + (i & 3) * 4 * kBlock),
+                               n_own & 1 ? pb[i >> 2] : pa[i >> 2], w.o[i & 3]);
+  }
+}
+
+// An item of 256 rows (WK = 1), or of 128 rows against two tiles a round (WK = 2: waves 0..3 work on the
+// first and waves 4..7 on the second).  256 rows take the tiles that all of them see whole as above;
+// what is left, and 128 rows, go tile by tile with the masks of their rows.
+template <typename T, int WK, bool OWN>
+__device__ inline void tile_item(const SharedArgs& a, const Source& src, const Item& it, char* lds) {
+  typedef typename Mma<T>::v8 v8;
+  constexpr int kRows = kWaves / WK;  // waves side by side
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hh = lane >> 5, wr = wave % kRows, wk = wave / kRows;
+  const int per_page = (src.T + kTile - 1) / kTile;
+  const int n_tiles = steps_of(src, it.n_keys, kTile, per_page);
+  const int t0 = share_of(n_tiles, it.split, it.n_split), n_own = share_of(n_tiles, it.split + 1, it.n_split) - t0;
+  // the tiles that go ahead of the others; a few are not worth the start
+  int n_open = 0;
+  if constexpr (WK == 1) {
+    const int whole = it.open >= it.n_keys ? n_tiles : it.open / src.T * per_page + it.open % src.T / kTile;
+    n_open = whole - t0 < n_own ? whole - t0 : n_own;
+    if (OWN && n_open < 4) n_open = 0;
+  }
+  TileWalk walk, ahead;  // at the tile that loads last
+  if (n_own > 0) {       // the page lists load while the rows are looked up
+    walk.start(it, per_page, t0);
+    if (WK == 1) ahead.start(it, per_page, t0);
+  }
+  const bool busy = it.m0 + 32 * wr < it.m1;  // the wave has rows at all
+  const bool mine = it.m0 + 32 * wr + n < it.m1;
+  const int m = all_rows(a, it, mine ? it.m0 + 32 * wr + n : it.m0);
+  int b, l, gh;
+  row_of(a, m, b, l, gh);
+  const int lim = OWN ? keys_seen(it, l) : it.n_keys;
+  TileState<T> w;
+  tile_begin(w, a, it, m, hh);
+  int klane, vlane, kpiece[4], vpiece[4];
+  tile_lanes(src, wave, lane, klane, vlane, kpiece, vpiece);
+  if constexpr (WK == 1) {
+    if (n_open > 0) {
+      open_tiles<T>(w, ahead, walk, a, src, it, n_open, busy, wave, klane, vlane, kpiece, vpiece, lds);
+      if (n_open < n_own) {
+        walk.start(it, per_page, t0 + n_open);
+        __builtin_amdgcn_s_barrier();  // everybody is done with what lies in LDS
+        asm volatile("" ::: "memory");
+      }
     }
   }
-  tile_end(w, a, it, m, mine, hh, over_groups_sum(w.sum, 32));
+  const int n_rest = WK == 2 || OWN ? n_own - n_open : 0;
+  const int64_t head_size = (int64_t)src.Tp * kHeadDim;
+  TileAt ring[kRing - WK];  // the tiles in use and those on their way
+  auto stage = [&](TileAt& x, int t) {
+    if (t == 0) walk.first();
+    else walk.next();
+    x = walk.at(src, it, a.heads, head_size);
+    lds_char* const to = load_target(lds + (t & (kRing - 1)) * 32 * kBlock);
+    stage_k<T>(src, x, klane, to, wave);
+    stage_v<T>(src, x, vlane, to + 16 * kBlock, wave);
+  };
+#pragma unroll
+  for (int i = 0; i < kRing - WK; ++i) {
+    ring[i] = TileAt{};
+    if (i < n_rest) stage(ring[i], i);
+  }
+  // the queries' own wait, ahead of the loop's counted ones
+#pragma unroll
+  for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
+  for (int t = 0; t < n_rest; t += WK) {
+    // This round's tiles have landed (a wave's loads land in order: what was issued after them may
+    // still be under way), and everybody is done with the round before, whose buffers load next.
+    constexpr int kLoads = 4;  // of a wave and tile
+    if (WK == 1 && t + 2 < n_rest) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+    else if (WK == 1 && t + 1 < n_rest) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const TileAt cur = WK == 2 && wk == 1 ? ring[1] : ring[0];
+#pragma unroll
+    for (int i = 0; i + WK < kRing - WK; ++i) ring[i] = ring[i + WK];
+#pragma unroll
+    for (int i = 0; i < WK; ++i)
+      if (t + kRing - WK + i < n_rest) stage(ring[kRing - 2 * WK + i], t + kRing - WK + i);
+    const char* const kt = lds + ((t + wk) & (kRing - 1)) * 32 * kBlock;
+    const char* const vt = kt + 16 * kBlock;
+    if (busy && t + wk < n_rest) {
+      f32x16 sc[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sc[i & 1] = Mma<T>::mul(*reinterpret_cast<const v8*>(kt + kpiece[(i >> 1) & 3] + ((i >> 3) * 8 + (i & 1) * 4) * kBlock),
+                                w.q[i >> 1], sc[i & 1]);
+      ahead_of_products();
+      const bool partial = OWN && cur.key0 + cur.valid > it.open, masked = cur.valid < kTile || partial;
+      if (masked) {
+        const int seen = lim - cur.key0;
+        int most = (seen < cur.valid ? seen : cur.valid) - 8 * hh;
+        asm volatile("" : "+v"(most));  // keeps this a branch: most tiles have nothing to mask
+        mask_keys(sc, most, OWN ? 0 : cur.valid, std::make_integer_sequence<int, 4>{});
+      }
+      v8 p[4];
+      const float sum = probs<T>(sc, a.c, w.mx == -INFINITY ? 0.0f : w.mx, p);
+      settle<T>(w, sc, a.c, sum, p, !(sum <= 256.0f) || w.mx == -INFINITY);
+      if (masked) {
+        masked_pv<T, OWN>(w, cur, partial, vt, vpiece, p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          w.o[i & 3] = Mma<T>::mul(*reinterpret_cast<const v8*>(vt + vpiece[i >> 2] + (i & 3) * 4 * kBlock), p[i >> 2],
+                                   w.o[i & 3]);
+        ahead_of_products();
+      }
+    }
+  }
+  float sum = over_groups_sum(w.sum, 32);
+  if constexpr (WK == 2) {  // the two halves of the waves join through LDS
+    float* const at = reinterpret_cast<float*>(lds) + wr * 66 * 64 + lane;
+    __syncthreads();
+    if (wk == 1) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) at[i * 64] = w.o[i >> 4][i & 15];
+      at[64 * 64] = w.mx;
+      at[65 * 64] = sum;
+    }
+    __syncthreads();
+    if (wk == 1) return;
+    const float m2 = at[64 * 64], l2 = at[65 * 64];
+    const float top = fmaxf(w.mx, m2), ms = top == -INFINITY ? 0.0f : top;
+    const float x = __builtin_amdgcn_exp2f(w.mx - ms), y = __builtin_amdgcn_exp2f(m2 - ms);
+    w.mx = top;
+    sum = sum * x + l2 * y;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) w.o[i >> 4][i & 15] = w.o[i >> 4][i & 15] * x + at[i * 64] * y;
+  }
+  tile_end(w, a, it, m, mine, hh, sum);
 }
+
 
 __device__ inline void prefix_keys(const SharedArgs& a, Item& it) {
   it.list = a.pre_pages;
@@ -1286,8 +1291,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
     it.m0 = (unit - pair * blocks) * R;
     it.m1 = it.m0 + R < rows ? it.m0 + R : rows;
     prefix_keys(a, it);
-    if constexpr (PK == 1) prefix_item<T>(a, a.pre, it, lds);
-    else if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
+    if constexpr (PK) tile_item<T, PK, false>(a, a.pre, it, lds);
     else stream_item<T, false>(a, a.pre, it, kWaves, reinterpret_cast<float*>(lds));
     return;
   }
