@@ -129,7 +129,9 @@ __device__ inline void v_tile(const AppendPagesArgs& a, int unit, uint32_t (&buf
 }
 
 // Workgroups [0, n_unit_groups): 16 (token, head block) units each of q and then of k; the rest:
-// V, a tile of a page each.
+// V, a tile of a page each.  One launch does all of it: it is bound by bytes where there are many tokens
+// (eight padded sequences of up to 1560 tokens, 24 heads, zero rows of the padding included: 156 MB read and
+// 187 written in 66 us, 5.1 TB/s) and by its launch where there are few (3.9 us for one token of 12 heads, 5.6 for 64 of 32 + 8).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
   __shared__ uint32_t buf[kTile][65];
@@ -203,16 +205,30 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
 // order that makes the probabilities a lane holds those of neighbouring keys: they are the second
 // product's B operand as they stand, and its A operand is 16 B pieces of V rows.
 //
-// Few rows (at most 16 of a key head) stream: each of 4 waves takes its own share of the keys, K and
-// V straight from memory to registers, bound by bytes.  More rows share: 4 waves of 32 rows read
-// tiles of 64 keys that the workgroup stages in LDS, bound by the matrix cores.
+// A workgroup of 8 waves has a CU to itself (the tiles take 128 KB of its LDS, a wave up to 256 registers)
+// and works on one item: some rows of a key head against a share of the keys.  By the number of rows:
+//  * up to 16 stream: every wave takes its own share of the keys, K and V straight from memory to
+//    registers.  Bound by bytes: 21 sequences, 12 heads, 7808 keys each, 1 GB in 197 us, 5.1 TB/s.
+//  * up to 128: two tiles of 64 keys a round in LDS, four waves of 32 rows on each.  Bound by
+//    bytes up to some 64 rows (the same keys 176 us, 5.7 TB/s with some of it in the last cache); 213 us at
+//    128 rows.
+//  * more: 256 rows, one tile a round, software-pipelined.  Bound by the matrix cores and the power they
+//    draw: 1024 rows of 8 heads against 131072 keys 521 us, 1.05 PFLOP/s, where a large library product
+//    reaches 1.35; a tile takes 1.45 us with half of the CUs at work and 2.0 with all.  Each 32 x 16 operand
+//    is read from LDS by the wave that multiplies it, 256 KB a tile, which takes LDS as long as the products
+//    take the matrix cores.
+// The limits, both sides measured (us): 4 sequences of 16 rows, 12 heads, 7808 keys 41.6 streaming, 43.0 by
+// tiles, and 20 rows of 8 heads against 32760 keys 46.6 and 39.2; 128 rows of those sequences 48.5 by two
+// tiles a round, 54.9 by one, and 160 rows 79.6 and 71.6.
 // ---------------------------------------------------------------------------------------------
 constexpr int kWaves = 8;    // of a workgroup: one workgroup a CU, two waves a SIMD
 // rows of a work item that streams (0) or goes by 1 or 2 tiles a round, and how many rows go
 constexpr int kind_rows(int kind) { return kind == 0 ? 16 : 32 * kWaves / kind; }
 constexpr int kind_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 128 ? 2 : 1; }
 constexpr int kStep = 32;    // keys of a streaming step
-constexpr int kCompact = 1024;  // sequences whose padding rows a prefix by tiles leaves out
+// Sequences whose padding rows a prefix by tiles leaves out (a search in LDS a lane): 32 sequences of up to
+// 16 tokens, half of them padding, 32 + 8 heads, against 32760 keys 342 -> 200 us.
+constexpr int kCompact = 1024;
 constexpr float kSlack = 8;  // the running maximum may lag the true one by 2^8 (see below)
 
 struct Source {
@@ -646,7 +662,6 @@ __device__ inline void stream_both(const SharedArgs& a, const Item& pre, const I
 // c ^ (r / 2) % 8 of the row in memory: the 16 lanes that an operand read serves at once then fall on
 // different banks.  Row i of a K operand is key 16 (i / 16) + 8 ((i / 4) % 2) + 4 ((i / 8) % 2) + i % 4
 // of its 32: the 16 scores of lane (n, hh) are then row n's keys 8 hh .. 8 hh + 7 and 16 + 8 hh .. + 7.
-//
 constexpr int kBlock = 1024;  // bytes that a wave's direct load fills
 constexpr int kRing = 4;  // tiles in LDS
 constexpr int kTileLds = kRing * 32 * kBlock;
@@ -909,12 +924,12 @@ __device__ inline void drop_keys(char* vt, int valid) {
   }
 }
 
-// 256 rows against keys that all of them see, software-pipelined: round t holds the scores of tile t + 1, the probabilities
-// of tile t and the second product of tile t - 1, 32 products with a slice of the softmax after each, so
-// that the matrix cores and the vector units work at the same time.  K and V have rings of their own:
-// K t + 1 and V t - 1 are in use while K t + 2 .. t + 4 and V t .. t + 2 are on their way.
-// Tiles [t0, t0 + n_own) of the item's keys, which all rows see as far as they exist; kw and vw have started
-// at t0.
+// 256 rows against n_own tiles of keys that all of them see as far as they exist, software-pipelined: round t
+// holds the scores of tile t + 1, the probabilities of tile t and the second product of tile t - 1, 32
+// products with a slice of the softmax after each, so that the matrix cores and the vector units work at the
+// same time (753 -> 700 us for 1024 rows of 8 heads against 131072 keys and own pages; one after the other,
+// with only the other wave of a SIMD to overlap, before).  K and V have rings of their own: K t + 1 and V t - 1
+// are in use while K t + 2 .. t + 4 and V t .. t + 2 are on their way.  kw and vw have started at tile 0.
 template <typename T>
 __device__ inline __attribute__((always_inline)) void open_tiles(TileState<T>& w, TileWalk& kw, TileWalk& vw, const SharedArgs& a, const Source& src,
                                   const Item& it, int n_own, bool busy, int wave, int klane, int vlane,
@@ -1233,7 +1248,8 @@ __device__ inline void own_keys(const SharedArgs& a, Item& it, int b, bool none)
 }
 
 // The prefix's work items first, dealt so that the row blocks of one (key head, split) run one after
-// another on one XCD and share its L2; then every sequence's own pages.  PK, OK: how the prefix and the
+// another on one XCD and share its L2 (interleaved with the others 765 -> 947 us at 1024 rows of 8 heads
+// against 131072 keys); then every sequence's own pages.  PK, OK: how the prefix and the
 // own pages go (0: streaming, else tiles a round).
 template <typename T, int PK, int OK>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArgs a) {
@@ -1319,7 +1335,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_shared_kernel(SharedArg
 }
 
 // The join of up to kFewParts parts: half a wave per (row, key head), a lane four channels, all parts'
-// values under way at once.
+// values under way at once (3 parts of 18720 rows, 29 MB, 7.6 us; a wave a row as below 13.3).
 constexpr int kFewParts = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void merge_few_kernel(SharedArgs a, int n_parts) {
@@ -1359,7 +1375,7 @@ __global__ __launch_bounds__(256) void merge_few_kernel(SharedArgs a, int n_part
 }
 
 // One wave per (row, key head).  Lane p weighs part p (64 parts at a time); then each half of the wave
-// adds every other part, a lane four channels, with four loads in flight.
+// adds every other part, a lane four channels, with four loads in flight (17 parts of 1024 rows 6.4 us).
 template <typename T>
 __global__ __launch_bounds__(256) void merge_kernel(SharedArgs a, int n_parts) {
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
