@@ -406,6 +406,140 @@ def test_many_splits_and_many_rows(gpu):
                 assert float(err.max()) <= 0, (b, i, h, float(err.max()))
 
 
+def _listed(kpool, vpool, page, ids, tokens):
+    """float64 K, V [H, tokens, D] of a page list on the GPU, and which tokens are there."""
+    at = ids.long().clamp(0, kpool.shape[0] - 1)
+    h = kpool.shape[2]
+    k = kpool[at, 0, :, :page].transpose(0, 1).reshape(h, -1, D)[:, :tokens].double()
+    v = vpool[at, 0, :, :, :page].permute(1, 0, 3, 2).reshape(h, -1, D)[:, :tokens].double()
+    there = ((ids >= 0) & (ids < kpool.shape[0])).repeat_interleave(page)[:tokens]
+    return torch.where(there[:, None], k, 0.0), torch.where(there[:, None], v, 0.0), there
+
+
+def _check_sequence(got, q, k, v, seen, dtype, what):
+    """One sequence's rows [L, Hq, D] against float64 attention over the keys that ``seen`` [L, T] names."""
+    n, hq, _ = q.shape
+    h = k.shape[0]
+    qs = q.double().reshape(n, h, hq // h, D).permute(1, 0, 2, 3).reshape(h, -1, D)
+    mask = seen.repeat_interleave(hq // h, 0)
+    s = (torch.bmm(qs, k.transpose(1, 2).contiguous()) * D ** -0.5).masked_fill(~mask, -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)  # rows that see nothing
+    o, a = torch.bmm(p, v), torch.bmm(p, v.abs())
+    size = (torch.bmm(qs.abs(), k.abs().transpose(1, 2).contiguous()) * D ** -0.5).masked_fill(~mask, 0.0)
+    e = HALF[dtype] * (a + o.abs()) * (1 + 2.0**-6) + TINY[dtype]
+    if dtype == F16:
+        e = e + 2.0**-25 * torch.bmm(mask.double().expand(h, -1, -1).contiguous(), v.abs())
+    bar = e + U * (320 * size.amax(-1, keepdim=True) + 64 + k.shape[1] / 64) * a
+    g = got.double().reshape(n, h, hq // h, D).permute(1, 0, 2, 3).reshape(h, -1, D)
+    assert torch.isfinite(g).all(), what
+    over = float(((g - o).abs() - bar).max())
+    assert over <= 0, (what, over)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("page,hole", [(64, None), (64, 4), (48, 3), (100, 0), (390, 1), (1, 70)])
+def test_prefix_of_any_length(gpu, page, hole, dtype):
+    """720 rows against prefixes from one key to many tiles a workgroup, whole pages and cut ones, one of
+    them not there; what lies behind the prefix's last token is no key, whatever it holds."""
+    b, n, hkv, group, longest = 9, 40, 32, 2, 130 if page == 1 else 1700
+    n_pre, own = -(-longest // page), 64
+    kpool, vpool = (t.to(gpu) for t in _pools(b, hkv, own, dtype, "cpu", 201))
+    kpre, vpre = (t.to(gpu) for t in _pools(n_pre, hkv, page, dtype, "cpu", 203))
+    ids = torch.randperm(n_pre, generator=_gen(205)).int().to(gpu)
+    if hole is not None:
+        ids[hole] = -1
+    tables, lengths = torch.arange(b, dtype=torch.int32, device=gpu)[:, None].contiguous(), [n + i for i in range(b)]
+    q = torch.randn(b, n, hkv * group, D, generator=_gen(206)).to(dtype).to(gpu)
+    for prefix in (1, 63, 64, 65, 129, 200, 330, 450, 700, 1100, longest):
+        if prefix > longest:
+            continue
+        print("prefix", page, prefix, dtype, flush=True)
+        last, o = int(ids[(prefix - 1) // page]), (prefix - 1) % page + 1
+        kp, vp = kpre.clone(), vpre.clone()
+        if last >= 0:
+            kp[last, 0, :, o:] = float("inf")
+            vp[last, 0, :, :, o:] = float("nan")
+        got = attend_shared(q, kpool, vpool, tables, _i32(lengths, gpu), page_tokens=own,
+                            prefix_pages=ids, prefix_tokens=prefix, prefix_pools=(kp, vp, page))
+        k0, v0, there = _listed(kp, vp, page, ids, prefix)
+        for i in range(b):
+            k1, v1, _ = _listed(kpool, vpool, own, tables[i], lengths[i])
+            row = torch.arange(n, device=gpu)[:, None]
+            seen = torch.cat((there.expand(n, -1), torch.arange(lengths[i], device=gpu) <= lengths[i] - n + row), 1)
+            _check_sequence(got[i], q[i], torch.cat((k0, k1), 1), torch.cat((v0, v1), 1), seen, dtype, (prefix, i))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("page,padded,prefix", [(64, False, 0), (100, True, 0), (390, False, 70), (48, True, 70)])
+def test_many_rows_of_own_keys(gpu, page, padded, prefix, causal):
+    """150 rows of 16 sequences against own keys of many tiles a workgroup: tiles that all rows see, then
+    those of the causal limit; cut pages, pages that are not there, padding, keys behind the length."""
+    b, n, hkv = 16, 150, 16
+    width = -(-1100 // page)
+    kpool, vpool = (t.to(gpu) for t in _pools(b * width + 2, hkv, page, BF, "cpu", 211))
+    tables = torch.randperm(b * width, generator=_gen(213)).int().reshape(b, width).to(gpu)
+    ids = _i32([b * width, b * width + 1], gpu)
+    lengths = [150 + 61 * i for i in range(b)]  # 150 .. 1065
+    new = [n - 9 * i for i in range(b)] if padded else None
+    tables[3, 1] = -1
+    tables[7, 0] = b * width + 2
+    for i, length in enumerate(lengths):
+        p, o = int(tables[i, length // page]), length % page
+        if 0 <= p < kpool.shape[0]:
+            kpool[p, 0, :, o:] = float("inf")
+            vpool[p, 0, :, :, o:] = float("nan")
+    q = torch.randn(b, n, hkv, D, generator=_gen(214)).to(BF).to(gpu)
+    pre = min(prefix, 2 * page)
+    got = attend_shared(q, kpool, vpool, tables, _i32(lengths, gpu), page_tokens=page, causal=causal,
+                        prefix_pages=ids, prefix_tokens=pre, new_lens=None if new is None else _i32(new, gpu))
+    k0, v0, t0 = _listed(kpool, vpool, page, ids, pre)
+    for i in range(b):
+        m = n if new is None else new[i]
+        k1, v1, t1 = _listed(kpool, vpool, page, tables[i], lengths[i])
+        row = torch.arange(m, device=gpu)[:, None]
+        limit = lengths[i] - m + row if causal else lengths[i] + 0 * row
+        seen = torch.cat((t0.expand(m, -1), t1 & (torch.arange(lengths[i], device=gpu) <= limit)), 1)
+        _check_sequence(got[i, :m], q[i, :m], torch.cat((k0, k1), 1), torch.cat((v0, v1), 1), seen, BF, i)
+        assert not got[i, m:].any()
+
+
+def test_values_at_the_limit_of_many_rows(gpu):
+    """150 rows over 600 own keys: an infinity and a NaN in V of a token reach the rows that see it and no
+    earlier ones, behind the tiles that all rows see."""
+    b, n, hkv, page = 16, 150, 16, 64
+    kpool, vpool = (t.to(gpu) for t in _pools(b * 10, hkv, page, BF, "cpu", 221))
+    tables = torch.arange(b * 10, dtype=torch.int32, device=gpu).reshape(b, 10)
+    q = torch.randn(b, n, hkv, D, generator=_gen(222)).to(BF).to(gpu)
+
+    def run():
+        return attend_shared(q, kpool, vpool, tables, _i32([600] * b, gpu), page_tokens=page)
+
+    clean = run()
+    at = 100  # row 100's own token
+    p, o = (450 + at) // page, (450 + at) % page
+    vpool[tables[:, p].long(), 0, :, 5, o], vpool[tables[:, p].long(), 0, :, 77, o] = float("inf"), float("nan")
+    got = run()
+    assert torch.equal(got[:, :at], clean[:, :at])
+    assert torch.isinf(got[:, at:, :, 5]).all() and torch.isnan(got[:, at:, :, 77]).all()
+    rest = [c for c in range(D) if c not in (5, 77)]
+    assert torch.equal(got[:, at:][..., rest], clean[:, at:][..., rest])
+
+
+@pytest.mark.parametrize("prefix,length,new,rows,hq", [(100, 1, None, 1, 4), (129, 130, None, 3, 4), (64, 0, 0, 2, 2),
+                                                       (1, 64, 2, 4, 8), (300, 90, None, 1, 2)])
+def test_single_sequence_with_few_keys(gpu, prefix, length, new, rows, hq):
+    """One sequence whose prefix and own keys one workgroup takes, with a page of each that is not there."""
+    page, hkv = 48, 2
+    kpool, vpool = _pools(16, hkv, page, BF, "cpu", 231)
+    tables, ids = torch.tensor([[3, -1, 5, 6]], dtype=torch.int32), [7, 16, 9, 10, 11, 12, 13]
+    q = torch.randn(1, rows, hq, D, generator=_gen(232)).to(BF)
+    new = None if new is None else [new]
+    want, bar = _attention(q, (kpool, vpool, page, tables), [length], new, True, (kpool, vpool, page, ids, prefix))
+    got = attend_shared(q.to(gpu), kpool.to(gpu), vpool.to(gpu), tables.to(gpu), _i32([length], gpu), page_tokens=page,
+                        prefix_pages=_i32(ids, gpu), prefix_tokens=prefix, new_lens=None if new is None else _i32(new, gpu))
+    _check(got, want, bar)
+
+
 @pytest.mark.parametrize("b,rows,prefix", [(150, 1, 0), (150, 2, 100), (1100, 2, 64)])
 def test_many_short_sequences(gpu, b, rows, prefix):
     """More sequences than CUs (several share a workgroup) and more than the 1024 whose padding rows
