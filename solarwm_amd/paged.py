@@ -41,11 +41,12 @@ def _check_pools(what: str, kpool: torch.Tensor, vpool: torch.Tensor, page_token
     if page_tokens <= 0:
         raise ValueError(f"{what}page_tokens must be positive, got {page_tokens}")
     tp = kernels.padded_tokens(page_tokens)
-    if kpool.dim() != 5 or kpool.shape[1] != 1:
+    shape = kpool.shape
+    if len(shape) != 5 or shape[1] != 1:
         raise ValueError(f"{what}pools must be K [pages, 1, H, Tp, 128] / V [pages, 1, H, 128, Tp], got "
-                         f"{tuple(kpool.shape)}")
-    n, _, h = kpool.shape[:3]
-    if kpool.shape != (n, 1, h, tp, HEAD_DIM) or vpool.shape != (n, 1, h, HEAD_DIM, tp):
+                         f"{tuple(shape)}")
+    n, _, h, rows, width = shape
+    if rows != tp or width != HEAD_DIM or vpool.shape != (n, 1, h, HEAD_DIM, tp):
         raise ValueError(f"{what}pool shapes {tuple(kpool.shape)} / {tuple(vpool.shape)} do not match "
                          f"page_tokens={page_tokens} (Tp = {tp})")
     if kpool.dtype != dtype or vpool.dtype != dtype:
@@ -74,9 +75,10 @@ def _check_out(out: torch.Tensor, q: torch.Tensor) -> None:
 
 def _set_pages(d, kpool, vpool, n_pages, page_tokens, tables, lengths, new_lens, batch) -> None:
     """The fields that both descriptors share."""
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != batch:
-        raise ValueError(f"tables must be int32 [{batch}, pages], got {tables.dtype} {tuple(tables.shape)}")
-    if tables.shape[1] > 1 and tables.stride(1) != 1:
+    shape, stride = tables.shape, tables.stride()
+    if tables.dtype != torch.int32 or len(shape) != 2 or shape[0] != batch:
+        raise ValueError(f"tables must be int32 [{batch}, pages], got {tables.dtype} {tuple(shape)}")
+    if shape[1] > 1 and stride[1] != 1:
         raise ValueError("tables must be contiguous in their last dimension")
     _int32_vector("lengths", lengths, batch)
     if new_lens is not None:
@@ -84,8 +86,8 @@ def _set_pages(d, kpool, vpool, n_pages, page_tokens, tables, lengths, new_lens,
         d.new_lens = new_lens.data_ptr()
     d.k_pool, d.v_pool = kpool.data_ptr(), vpool.data_ptr()
     d.dtype, d.n_pages, d.page_tokens = kernels.dtype_code(kpool.dtype), n_pages, page_tokens
-    d.tables, d.table_width = tables.data_ptr(), tables.shape[1]
-    d.table_stride = tables.stride(0) if batch > 1 else 0
+    d.tables, d.table_width = tables.data_ptr(), shape[1]
+    d.table_stride = stride[0] if batch > 1 else 0
     d.lengths, d.head_dim = lengths.data_ptr(), HEAD_DIM
 
 
@@ -161,8 +163,9 @@ def append_pages(
     d.k_sb, d.k_st, d.k_sh = strides("k", k)
     d.v_sb, d.v_st, d.v_sh = strides("v", v)
     if cos is not None:
-        d.cos, d.sin, d.half, d.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0]
-        d.cos_stride = cos.stride(0) if cos.shape[0] > 1 else cos.shape[1]
+        d.cos, d.sin = cos.data_ptr(), sin.data_ptr()
+        d.table_rows, d.half = cos.shape
+        d.cos_stride = cos.stride(0) if d.table_rows > 1 else d.half
     if positions is not None:
         if cos is None:
             raise ValueError("positions without cos and sin")

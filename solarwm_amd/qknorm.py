@@ -38,10 +38,10 @@ def head_norm_spec(name: str, norm) -> tuple[torch.Tensor | None, float]:
     a ``(weight, eps)`` pair."""
     weight, eps = norm if isinstance(norm, tuple) else (norm.weight, norm.eps)
     if weight is not None:
-        if weight.dim() != 1 or weight.shape[0] != HEAD_DIM or weight.dtype not in _FLOATS:
+        if weight.shape != (HEAD_DIM,) or weight.dtype not in _FLOATS:
             raise ValueError(f"{name} weight must be [{HEAD_DIM}] (one head), float32, bfloat16 or "
                              f"float16; got {weight.dtype} {tuple(weight.shape)}")
-        if weight.stride(0) != 1:
+        if not weight.is_contiguous():
             raise ValueError(f"{name} weight must be contiguous")
     return weight, float(eps)
 
@@ -56,8 +56,9 @@ def strides(name: str, t: torch.Tensor) -> tuple[int, int, int]:
 
 
 def check_heads(name: str, t: torch.Tensor, dtypes) -> None:
-    if t.dim() != 4 or t.shape[3] != HEAD_DIM:
-        raise ValueError(f"{name} must be [B, L, H, {HEAD_DIM}], got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM:
+        raise ValueError(f"{name} must be [B, L, H, {HEAD_DIM}], got {tuple(shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} dtype {t.dtype} unsupported ({', '.join(map(str, dtypes))})")
 
@@ -67,13 +68,14 @@ def check_tables(cos, sin) -> None:
         raise ValueError("give cos and sin together")
     if cos is None:
         return
-    if cos.dim() != 2 or cos.shape != sin.shape:
+    shape, stride = cos.shape, cos.stride()
+    if len(shape) != 2 or sin.shape != shape:
         raise ValueError(f"cos / sin must be [positions, pairs], got {tuple(cos.shape)} / {tuple(sin.shape)}")
-    if cos.shape[1] % 8 or not 8 <= cos.shape[1] <= HEAD_DIM // 2:
-        raise ValueError(f"cos / sin need 8, 16 .. {HEAD_DIM // 2} columns (one per rotated pair), got {cos.shape[1]}")
+    if shape[1] % 8 or not 8 <= shape[1] <= HEAD_DIM // 2:
+        raise ValueError(f"cos / sin need 8, 16 .. {HEAD_DIM // 2} columns (one per rotated pair), got {shape[1]}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("cos / sin must be float32")
-    if cos.stride(1) != 1 or sin.stride() != cos.stride():
+    if stride[1] != 1 or sin.stride() != stride:
         raise ValueError("cos and sin must share strides, with unit column stride")
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise ValueError("cos / sin take no gradient")
@@ -92,13 +94,14 @@ def check_positions(positions, batch: int, rows: int) -> tuple[int, int]:
 
 def same_device(names: tuple[str, ...], tensors: tuple) -> None:
     """Every tensor that is given is on the GPU of the first."""
-    device = tensors[0].device
-    if device.type == "cuda":
+    index = tensors[0].get_device()  # -1: not on a GPU
+    if index >= 0:
         for t in tensors:
-            if t is not None and t.device != device:
+            if t is not None and t.get_device() != index:
                 break
         else:
             return
+    device = tensors[0].device
     for name, t in zip(names, tensors):
         if t is not None:
             kernels._require_cuda(name, t)
