@@ -1490,15 +1490,15 @@ struct SharedPlan {
 // Key splits, and waves of a streaming item, by what they are estimated to take (microseconds, as
 // measured on MI355X).  A workgroup has a CU to itself, so what counts is rounds of workgroups.  A
 // workgroup takes kFixed to start and end (7.5 us with two steps).  A tile against 256 rows takes 1.45 us
-// of a prefix and 1.7 of own pages while half of the CUs work, and 2.0 and 2.2 when all do (the clock
-// follows the power), two tiles against 128 rows 2.3.  A streaming CU reads 38 GB/s (64 keys in 0.86 us),
+// of a prefix and 1.55 of own pages while half of the CUs work, and 2.0 and 2.45 when all do (the clock
+// follows the power, and own pages are shared by no one), two tiles against 128 rows 2.3.  A streaming CU reads 38 GB/s (64 keys in 0.86 us),
 // and the whole chip 4.6 TB/s.  Several parts cost kMerge and the bytes of their partial results.
 void choose_splits(const skv_attend_shared_desc* d, int64_t M, int64_t cu, int64_t pre_items, int64_t pre_tiles,
                    int64_t own_items, int64_t own_tiles, SharedPlan* p) {
   constexpr double kFixed = 7.0, kBytes = 4.6e6, kMerge = 7.0, kTileBytes = 32768.0;
   auto tile_cost = [](int kind, bool own, double busy) {
     const double over = busy < 0.5 ? 0.0 : (busy < 1.0 ? busy : 1.0) - 0.5;
-    return kind == 0 ? 0.86 : kind == 2 ? 1.15 : own ? 1.7 + over : 1.45 + 1.1 * over;
+    return kind == 0 ? 0.86 : kind == 2 ? 1.15 : own ? 1.55 + 1.8 * over : 1.45 + 1.1 * over;
   };
   // tables are as wide as their longest sequence gets: the average one holds half of that
   const double mean = 0.5 * own_tiles, longer = 0.75 * own_tiles;
