@@ -950,18 +950,29 @@ __device__ inline __attribute__((always_inline)) void open_tiles(TileState<T>& w
     else vw.next();
     stage_v<T>(src, vw.at(src, it, a.heads, head_size), vlane, load_target(vlds + (t & (kRing - 1)) * 16 * kBlock), wave);
   };
-#pragma unroll
-  for (int i = 0; i < kRing; ++i) {
-    valid[i] = kTile;
-    if (i < n_own) valid[i] = load_k(i);
-    if (i >= 2 && i - 2 < n_own) load_v(i - 2);
-  }
   // round 0 multiplies the tile in front of the first by nothing
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     *reinterpret_cast<u32x4*>(vlds + (kRing - 1) * 16 * kBlock + (threadIdx.x + i * 64 * kWaves) * 16) = u32x4{0u, 0u, 0u, 0u};
+  // The queries' own wait, ahead of the counted ones: they left with the page list, without which no key loads.
 #pragma unroll
   for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(w.q[st]));
+  if (n_own >= kRing) {
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) {
+      valid[i] = load_k(i);
+      if (i >= 2) load_v(i - 2);
+    }
+    asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)" ::: "memory");  // K 0; the other ten loads may be under way
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) {
+      valid[i] = kTile;
+      if (i < n_own) valid[i] = load_k(i);
+      if (i >= 2 && i - 2 < n_own) load_v(i - 2);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
   auto mask = [&](f32x16 (&sc)[2], int keys) __attribute__((always_inline)) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // keeps this a branch: most tiles have nothing to mask
@@ -976,7 +987,6 @@ __device__ inline __attribute__((always_inline)) void open_tiles(TileState<T>& w
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) pa[i][e] = (T)0.0f;
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   if (busy) {
