@@ -92,7 +92,7 @@ __device__ inline void v_tile(const AppendPagesArgs& a, int unit, uint32_t (&buf
   for (int i = 0; i < 4; ++i) {
     const int r = (tid >> 4) + 16 * i;
     if (r >= lo && r < hi) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(v + (row0 + r) * a.v_st);
+      const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v + (row0 + r) * a.v_st));
 #pragma unroll
       for (int e = 0; e < 4; ++e) buf[r][4 * c + e] = w[e];
     }
@@ -115,8 +115,8 @@ __device__ inline void v_tile(const AppendPagesArgs& a, int unit, uint32_t (&buf
     uint16_t* p0w = o + (int64_t)(2 * pair) * a.pg.Tp + r0;
     uint16_t* p1w = p0w + a.pg.Tp;
     if (r0 >= lo && r0 + 8 <= hi) {
-      *reinterpret_cast<u32x4*>(p0w) = even;
-      *reinterpret_cast<u32x4*>(p1w) = odd;
+      __builtin_nontemporal_store(even, reinterpret_cast<u32x4*>(p0w));
+      __builtin_nontemporal_store(odd, reinterpret_cast<u32x4*>(p1w));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
