@@ -64,7 +64,8 @@ __device__ inline Place place_of(const Pages& pg, int b, int64_t own) {
 }
 
 // V of the tokens that one 64-token tile of a page takes: rows in through LDS, out as pieces of 8
-// tokens of a channel (16 B) where all 8 are new, token by token at the ends.  A call of one token a
+// tokens of a channel (16 B) where all 8 are new, token by token at the ends, past the caches (as the rows of K
+// and q: together 77 -> 65 us for the eight sequences below).  A call of one token a
 // sequence goes the same way: a wave per token that stores its channels straight away takes as long
 // (128 sequences of 8 heads 6.6 us either way; 64 sequences of 8 tokens 9.9 us, by tiles 9.2).
 template <typename T>
@@ -130,8 +131,8 @@ __device__ inline void v_tile(const AppendPagesArgs& a, int unit, uint32_t (&buf
 
 // Workgroups [0, n_unit_groups): 16 (token, head block) units each of q and then of k; the rest:
 // V, a tile of a page each.  One launch does all of it: it is bound by bytes where there are many tokens
-// (eight padded sequences of up to 1560 tokens, 24 heads, zero rows of the padding included: 156 MB read and
-// 187 written in 66 us, 5.1 TB/s) and by its launch where there are few (3.9 us for one token of 12 heads, 5.6 for 64 of 32 + 8).
+// (eight padded sequences of up to 1560 tokens, 24 heads, zero rows of the padding included: 151 MB read and
+// 186 written in 58 us, 5.8 TB/s with part of the input in the last cache) and by its launch where there are few (3.9 us for one token of 12 heads, 5.6 for 64 of 32 + 8).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void append_pages_kernel(AppendPagesArgs a) {
   __shared__ uint32_t buf[kTile][65];

@@ -50,8 +50,8 @@ __device__ inline int64_t position(const QkArgs& a, int b, int row) {
 }
 
 // grid ceil(n_units / 16), block 256: 16 lanes per unit of kHeadBlock heads of one token, every
-// head's load issued before the first is worked on.  4680 tokens of 40 + 40 bf16 heads take 37.9 us, 5.1 TB/s,
-// what a large copy reaches; a few tokens 3.9 us, which is the launch.
+// head's load issued before the first is worked on.  4680 tokens of 40 + 40 bf16 heads take 35.1 us, 5.5 TB/s,
+// what a large copy reaches and part of the input in the last cache; a few tokens 3.9 us, which is the launch.
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a) {
   const int lane64 = threadIdx.x & 63;
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a) {
 // grid: n_groups_q workgroups that walk q's units, the rest k's.  A thread keeps the weight
 // gradient of its 8 channels over all its rows; the workgroup's 16 rows of sums meet in LDS and go
 // out as one row of partials, which qk_norm_dw_kernel adds in a fixed order.  16380 tokens of 24 + 24 bf16
-// heads: 604 MB in 127 us, 4.8 TB/s (the forward pass 73 us, 5.5 TB/s with part of it in the last cache).
+// heads: 604 MB in 108 us, 5.6 TB/s (the forward pass 67 us, 6.0 TB/s; part of the inputs in the last cache).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(QkArgs a) {
   __shared__ float part[16][kHeadDim];
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(QkArgs a) {
 }
 
 // grid (4, 2): 32 channels of q's or k's weight gradient from the workgroups' partials, in a fixed order
-// (2048 rows of partials 5 us).
+// (2048 rows of partials 4.4 us).
 __global__ __launch_bounds__(1024) void qk_norm_dw_kernel(QkArgs a, int n_groups_k) {
   __shared__ float part[128][33];
   const QkSide& s = blockIdx.y == 0 ? a.q : a.k;

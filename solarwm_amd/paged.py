@@ -6,7 +6,8 @@ sequence goes on in pages of its own:
 
 * a page is a frame slot with a batch of one, ``kernels.new_pools(n_pages, 1, heads, page_tokens,
   dtype, device)``: K ``[n_pages, 1, H, Tp, 128]``, V ``[n_pages, 1, H, 128, Tp]`` transposed, with
-  ``page_tokens`` tokens in use; the other functions on pools (``kernels.gather_frames``, ...) take
+  ``page_tokens`` tokens in use (attention works on 64 keys of a page at a time: multiples of 64 cost
+  least); the other functions on pools (``kernels.gather_frames``, ...) take
   them as they are, and a frame-slot cache with a batch of one is such a pool itself
   (:func:`history_pages`);
 * ``tables`` (int32 ``[B, W]`` on the GPU) names each sequence's pages in order, ``lengths`` (int32
